@@ -44,7 +44,7 @@ typedef enum { RD_BF16 = 0, RD_F16 = 1, RD_F32 = 2 } rd_dtype;
  * that crosses it (the attention plan, the realignment plan) or a workspace size changes.  A caller
  * compiled against this header compares rd_version() with RD_ABI_VERSION before its first call, so
  * that a stale build of the library is refused instead of being called with other arguments. */
-#define RD_ABI_VERSION 106
+#define RD_ABI_VERSION 107
 RD_API int rd_version(void);
 /* Message of the last failed call on this thread ("" if none). */
 RD_API const char* rd_last_error(void);
@@ -394,6 +394,70 @@ RD_API int rd_rope_verify_attention(const void* q, const int64_t* q_strides, con
                                     int n_kv_heads, int n_q, int kv_len, int head_dim, float scale,
                                     const uint64_t* bits, const int32_t* plan, void* workspace,
                                     size_t workspace_bytes, const int32_t* row_start, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * KV cache held in 4 or 8 bits.  (No counterpart in the reference, whose cache has the model's type.)
+ *
+ * A row of head_dim values (a multiple of 32, at most 256) is a record of rd_kv_quant_row_bytes(bits,
+ * head_dim) bytes: head_dim * bits / 8 code bytes, head_dim / 8 scale bytes, padding to a multiple of
+ * 16.  Eight consecutive values share a power of two 2^e (scale byte e + 127), the smallest with
+ * max |x| <= top * 2^e; their codes are x / 2^e rounded to the nearest, ties to even, saturated:
+ * bits 4: e2m1 (0 .5 1 1.5 2 3 4 6; value d in nibble d % 8 of its dword), top 7; bits 8: e4m3 without
+ * infinities (largest 448), top 464.  e is clamped so that every value is a finite number of dtype and
+ * exact in it (smallest e: -100, for RD_F16 -23 / -15).  A block that holds a NaN, an infinity or a
+ * number beyond dtype's largest has scale byte 255 and reads back as eight NaNs.
+ * The cache is a byte array (n_layers, 2, batch, n_kv_heads, max_len, row bytes), addressed like any
+ * other by rd_kv_unpack, rd_kv_compact, rd_kv_append and rd_kv_materialize with row_bytes = the record;
+ * below, cache_strides are HOST arrays of BYTE strides {batch, head, row}.
+ *
+ * rd_rope_append_quant: rd_rope_append into such rows.  k is rotated without intermediate rounding and
+ * the record is that of the exact rotated key; q_out is the rotated q rounded once (rd_rope_append
+ * rounds every product).  All other arguments as for rd_rope_append.
+ * rd_kv_quantize: rows x (batch, n_kv_heads, n_rows, head_dim), HOST element strides {batch, head, row},
+ * last dimension contiguous, into the cache rows [row0, row0 + n_rows) of one layer's keys or values.
+ * rd_kv_dequantize: the cache rows [row0, row0 + n_rows) as values of dtype (the type the rows were
+ * written from; rows start on 16-byte boundaries of `out`).
+ *
+ * rd_verify_attention_quant: rd_verify_attention over such rows; mask bits, plan and row_start as
+ * there.  spans: rd_attn_spans_ints(batch, n_q) int32 written by rd_attn_spans from the mask bits (once
+ * per forward: the first and one past the last key that 16 consecutive queries attend to).  A row that
+ * attends to nothing is written as zeros; keys nobody attends to may hold NaN blocks.  bf16 and fp16
+ * with head_dim 64 or 128 (q 16-byte aligned with strides that are multiples of 8 elements, out 8-byte
+ * aligned with strides that are multiples of 4) run on the MFMA kernel, everything else, or
+ * force_generic != 0, on the generic kernel.  workspace: rd_verify_attention_quant_workspace_bytes (0:
+ * none is needed, NULL will do), 256-byte aligned; each call needs one of its own while it runs.  Nothing
+ * in the library is shared between calls.  scale must be positive.  Rows of one slab must follow each
+ * other without gaps (cache_strides[2] = the record).  Limits: kv_len <= 2^23,
+ * n_q * n_heads / n_kv_heads <= 2^30. */
+RD_API size_t rd_kv_quant_row_bytes(int bits, int head_dim);
+RD_API int rd_rope_append_quant(const void* q, const int64_t* q_strides, const void* k,
+                                const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                                int dtype, int batch, int n_new, int n_heads, int n_kv_heads,
+                                int head_dim, const void* cos, const void* sin, int64_t table_rows,
+                                const int64_t* position_ids, int64_t pos_batch_stride, void* q_out,
+                                const int64_t* q_out_strides, void* k_cache, void* v_cache,
+                                const int64_t* cache_strides, int bits, int64_t row0, int64_t max_len,
+                                const int32_t* row_start, const int32_t* kv_row_shift, void* stream);
+RD_API int rd_kv_quantize(const void* x, const int64_t* x_strides, int dtype, int batch, int n_kv_heads,
+                          int64_t n_rows, int head_dim, int bits, void* cache,
+                          const int64_t* cache_strides, int64_t row0, int64_t max_len, void* stream);
+RD_API int rd_kv_dequantize(const void* cache, const int64_t* cache_strides, int bits, int dtype,
+                            int batch, int n_kv_heads, int64_t row0, int64_t n_rows, int head_dim,
+                            int64_t max_len, void* out, const int64_t* out_strides, void* stream);
+RD_API size_t rd_attn_spans_ints(int batch, int n_q);
+RD_API int rd_attn_spans(const uint64_t* bits, int batch, int n_q, int kv_len, int32_t* spans,
+                         void* stream);
+RD_API size_t rd_verify_attention_quant_workspace_bytes(int dtype, int batch, int n_heads,
+                                                        int n_kv_heads, int n_q, int kv_len,
+                                                        int head_dim);
+RD_API int rd_verify_attention_quant(const void* q, const int64_t* q_strides, const void* k_cache,
+                                     const void* v_cache, const int64_t* cache_strides, int bits,
+                                     int64_t max_len, void* out, const int64_t* o_strides, int dtype,
+                                     int batch, int n_heads, int n_kv_heads, int n_q, int kv_len,
+                                     int head_dim, float scale, const uint64_t* mask_bits,
+                                     const int32_t* plan, const int32_t* spans, void* workspace,
+                                     size_t workspace_bytes, int force_generic,
+                                     const int32_t* row_start, void* stream);
 
 /* ------------------------------------------------------------------------------------------
  * Causal mask from a padding mask: mask[b,i,j] = (j <= kv_len - query_len + i) && padding[b,j].

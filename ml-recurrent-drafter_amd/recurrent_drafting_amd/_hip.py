@@ -20,7 +20,7 @@ import sys
 _DEFAULT_LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libredrafter_hip.so")
 _LIB_PATH = os.environ.get("RD_HIP_LIBRARY") or _DEFAULT_LIB_PATH
 _lib = None
-ABI_VERSION = 106  # RD_ABI_VERSION of include/redrafter_hip.h that _PROTOTYPES below was written against
+ABI_VERSION = 107  # RD_ABI_VERSION of include/redrafter_hip.h that _PROTOTYPES below was written against
 
 RD_BF16, RD_F16, RD_F32 = 0, 1, 2
 _DTYPES = {torch.bfloat16: RD_BF16, torch.float16: RD_F16, torch.float32: RD_F32}
@@ -71,6 +71,20 @@ _PROTOTYPES = {
         _I,
         [_P, _P, _P, _P, _P, _P, _P, _P, _L, _P, _L, _P, _P, _P, _L, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F,
          _P, _P, _P, _Z, _P, _P],
+    ),
+    "rd_kv_quant_row_bytes": (_Z, [_I, _I]),
+    "rd_rope_append_quant": (
+        _I,
+        [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P, _P, _L, _P, _L, _P, _P, _P, _P, _P, _I, _L, _L, _P, _P, _P],
+    ),
+    "rd_kv_quantize": (_I, [_P, _P, _I, _I, _I, _L, _I, _I, _P, _P, _L, _L, _P]),
+    "rd_kv_dequantize": (_I, [_P, _P, _I, _I, _I, _I, _L, _L, _I, _L, _P, _P, _P]),
+    "rd_attn_spans_ints": (_Z, [_I, _I]),
+    "rd_attn_spans": (_I, [_P, _I, _I, _I, _P, _P]),
+    "rd_verify_attention_quant_workspace_bytes": (_Z, [_I, _I, _I, _I, _I, _I, _I]),
+    "rd_verify_attention_quant": (
+        _I,
+        [_P, _P, _P, _P, _P, _I, _L, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _P, _P, _P, _P, _Z, _I, _P, _P],
     ),
     "rd_causal_mask": (_I, [_P, _I, _L, _I, _L, _L, _P, _P]),
     "rd_verify_row_stats": (_I, [_P, _I, _L, _L, _I, _I, _F, _F, _P, _I, _P]),
@@ -161,6 +175,17 @@ def stream():
     if _raw_stream is not None and _raw_device is not None:
         return _raw_stream(_raw_device())
     return torch.cuda.current_stream().cuda_stream
+
+
+def on_current_device(*tensors: torch.Tensor) -> None:
+    """Refuses tensors that are not on the current GPU: launches go to its current stream."""
+    current = torch.cuda.current_device() if tensors[0].is_cuda else None
+    for t in tensors:
+        if not t.is_cuda:
+            ptr(t)  # says what it thinks of host tensors
+        if t.device.index != current:
+            raise RuntimeError(f"tensor on {t.device}, but the current GPU is cuda:{current}: "
+                               "make the tensors' GPU the current one (torch.cuda.device)")
 
 
 def dtype_code(dt: torch.dtype) -> int:

@@ -10,12 +10,12 @@ from __future__ import annotations
 
 import ctypes as C
 import math
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 from typing import Optional
 
 import torch
 
-from . import _hip
+from . import _hip, kv_cache
 from .packed_rows import PackedRows
 
 
@@ -61,6 +61,9 @@ class PreparedMask:
     kv_len: int
     workspace: Optional[torch.Tensor] = None
     shifted: bool = False  # the plan was built with per-row cache shifts (kv_cache.Cache.shift)
+    # first and one past the last key that 16 consecutive queries attend to: made by the first attention
+    # over a cache in 4 or 8 bits that uses this mask, per stream ({stream handle: int32 tensor})
+    spans: dict = field(default_factory=dict)
 
 
 def prepare(mask: torch.Tensor, fix_empty_rows: bool = True, n_heads: int = 32,
@@ -106,11 +109,14 @@ def masked_attention(
     force_generic: bool = False,
     rows: Optional[PackedRows] = None,
 ) -> torch.Tensor:
-    """q (B, H, n_q, D) [any strides with D contiguous], k/v (B, Hkv, kv_len, D) strided views.
+    """q (B, H, n_q, D) [any strides with D contiguous], k/v (B, Hkv, kv_len, D) strided views, or the
+    kv_cache.QuantizedRows of a cache in 4 or 8 bits.
 
     Returns (B, n_q, H*D), i.e. already in the layout o_proj consumes.  With `rows`, q is
     (rows.rows, H, D), the query rows that exist (and the stand-in rows behind them, which are
     neither read nor written), and the result is (rows.rows, H*D)."""
+    if isinstance(k, kv_cache.QuantizedRows) or isinstance(v, kv_cache.QuantizedRows):
+        return _quantized_attention(q, k, v, prepared, scale, force_generic, rows)
     Bk, Hkv, kv_len, Dk = k.shape
     if rows is None:
         B, H, n_q, D = q.shape
@@ -153,6 +159,69 @@ def masked_attention(
     return out.view(B, n_q, H * D) if rows is None else out.view(rows.rows, H * D)
 
 
+def _spans(prepared: PreparedMask) -> torch.Tensor:
+    """The mask's span table, written on the current stream: kept for the later layers on that stream.
+    A table written while a graph is captured holds nothing before the replay, so it stays with its call."""
+    stream = _hip.stream()
+    spans = prepared.spans.get(stream)
+    capturing = torch.cuda.is_current_stream_capturing()
+    if spans is None or capturing:
+        lib = _hip.lib()
+        spans = torch.empty(lib.rd_attn_spans_ints(prepared.batch, prepared.n_q), dtype=torch.int32,
+                            device=prepared.bits.device)
+        _hip.check(lib.rd_attn_spans(_hip.ptr(prepared.bits), prepared.batch, prepared.n_q, prepared.kv_len,
+                                     _hip.ptr(spans), stream))
+        if not capturing:
+            prepared.spans[stream] = spans
+    return spans
+
+
+def _quantized_attention(q, k, v, prepared: PreparedMask, scale, force_generic, rows) -> torch.Tensor:
+    """masked_attention over the rows of a cache in 4 or 8 bits (rd_verify_attention_quant)."""
+    assert isinstance(k, kv_cache.QuantizedRows) and isinstance(v, kv_cache.QuantizedRows), "keys and values of one cache"
+    Bk, Hkv, kv_len, D = k.shape
+    if rows is None:
+        B, H, n_q, Dq = q.shape
+    else:
+        T, H, Dq = q.shape
+        B, n_q = rows.batch, rows.n
+        assert T == rows.rows
+    assert (Bk, D) == (B, Dq) and v.shape == k.shape and (v.bits, v.dtype, v.max_length) == (k.bits, k.dtype, k.max_length)
+    assert q.dtype == k.dtype, "queries in the type the cache was written from"
+    assert list(v.strides()) == list(k.strides())
+    assert (prepared.batch, prepared.n_q, prepared.kv_len) == (B, n_q, kv_len), "mask/plan mismatch"
+    _hip.on_current_device(q, k.records, v.records, prepared.bits)
+    if q.stride(-1) != 1:
+        q = q.contiguous()
+    if rows is None:
+        out = torch.empty((B, n_q, H, D), dtype=q.dtype, device=q.device)
+        q_strides = _strides3(q)
+        o_strides = _strides3(out.permute(0, 2, 1, 3))  # (B, H, n_q, D) strides
+    else:
+        out = torch.empty((rows.rows, H, D), dtype=q.dtype, device=q.device)
+        q_strides = (C.c_int64 * 3)(0, q.stride(1), q.stride(0))
+        o_strides = (C.c_int64 * 3)(0, out.stride(1), out.stride(0))
+    lib = _hip.lib()
+    dtype = _hip.dtype_code(q.dtype)
+    spans = _spans(prepared)
+    # partial results of keys cut into pieces: memory of this call alone, so that calls on several
+    # streams, or captured in several graphs, may share the mask
+    ws_bytes = lib.rd_verify_attention_quant_workspace_bytes(dtype, B, H, Hkv, n_q, kv_len, D)
+    workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
+    if shape_log is not None:
+        shape_log.append((B, n_q, kv_len, B * n_q if rows is None else rows.total))
+    _hip.check(
+        lib.rd_verify_attention_quant(
+            _hip.ptr(q), q_strides, _hip.ptr(k.records), _hip.ptr(v.records), k.strides(), k.bits, k.max_length,
+            _hip.ptr(out), o_strides, dtype, B, H, Hkv, n_q, kv_len, D,
+            float(scale if scale is not None else 1.0 / math.sqrt(D)), _hip.ptr(prepared.bits),
+            _hip.ptr(prepared.plan), _hip.ptr(spans), _hip.ptr(workspace), ws_bytes,
+            int(force_generic), _hip.ptr(rows.row_start) if rows is not None else None, _hip.stream(),
+        )
+    )
+    return out.view(B, n_q, H * D) if rows is None else out.view(rows.rows, H * D)
+
+
 def rope_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
                    position_ids: torch.Tensor, past_key_value, prepared: PreparedMask,
                    rows: Optional[PackedRows] = None, fused: Optional[bool] = None) -> torch.Tensor:
@@ -165,19 +234,18 @@ def rope_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch
 
     bf16 with head_dim 128 and at most 256 new tokens per row runs as ONE kernel (rd_rope_verify_attention: the attention kernel rotates
     its query rows in registers and writes the new cache rows itself before it reads them; q stays
-    as it was); anything else, or fused=False, runs kv_cache.rope_append (which rotates q in place)
+    as it was); anything else (a cache in 4 or 8 bits too), or fused=False, runs kv_cache.rope_append (which rotates q in place)
     and masked_attention.  Both give the same bits in the output and in the cache."""
-    from . import kv_cache  # (kv_cache does not import this module)
-
     key_view, value_view = past_key_value
     cache = key_view._cache
-    _, _, batch, n_kv_heads, max_length, head_dim = cache.shape
+    batch, n_kv_heads, _, head_dim = key_view.shape
+    max_length = cache.shape[4]
     n_heads = q.shape[-1] // head_dim
     lib = _hip.lib()
     owner = key_view._owner
     in_place = owner is not None and owner.rows_in_place
     can_fuse = bool(lib.rd_rope_verify_attention_eligible(_hip.dtype_code(q.dtype), n_heads, head_dim,
-                                                          prepared.n_q)) and prepared.shifted == in_place
+                                                          prepared.n_q)) and prepared.shifted == in_place and key_view.bits is None
     if fused is None:
         fused = can_fuse
     assert can_fuse or not fused, "no fused kernel for this dtype / head_dim / cache layout"

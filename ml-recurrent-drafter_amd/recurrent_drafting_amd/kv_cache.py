@@ -10,17 +10,62 @@ Rows in place: the reference re-right-aligns the whole live cache after every st
 column c of row b lives in cache row c - shift[b]; the re-alignment adds the change of the left
 padding to it, and `rope_append` and the attention subtract it.  `Cache.materialize()` moves the rows
 once to the reference's layout; `View.cat`, `View.slice` and `Cache.unpack` call it first.
+
+Rows in 4 or 8 bits: `Cache(..., bits=4)` holds every row as a record of small scaled floats (blocks
+of 8 values with a common power of two; include/redrafter_hip.h has the format), 80 or 144 bytes at
+head_dim 128 where bf16 takes 256.  Rows are rounded as they are written (`rope_append`, `View.append`,
+`View.cat`) and read back in the model's type by `View.slice` and `View.cat`; `rope_append` and
+`View.rows` hand out `QuantizedRows`, which `attention.masked_attention` reads as they are.  Moving rows
+(unpack, compact, materialize, rows in place) moves the records.
 """
 
 from __future__ import annotations
 
 import ctypes
+from dataclasses import dataclass
 from typing import Optional, Tuple
 
 import torch
 
 from . import _hip
 from .packed_rows import PackedRows
+
+
+@dataclass
+class QuantizedRows:
+    """Key or value rows of one layer of a cache held in 4 or 8 bits."""
+
+    records: torch.Tensor  # (batch, n_heads, length, record bytes) uint8, a view of the cache
+    bits: int
+    head_dim: int
+    dtype: torch.dtype  # the type the rows were rounded from and read back in
+    max_length: int  # rows of a slab of the cache behind the view
+
+    @property
+    def shape(self) -> Tuple[int, int, int, int]:
+        return (*self.records.shape[:3], self.head_dim)
+
+    def strides(self):
+        """Byte strides {batch, head, row} for the C ABI."""
+        r = self.records
+        return (ctypes.c_int64 * 3)(r.stride(0), r.stride(1), r.stride(2))
+
+    def read(self) -> torch.Tensor:
+        """The values, (batch, n_heads, length, head_dim) in `dtype`: exact, every value the records can
+        hold is a number of that type."""
+        batch, n_heads, length, _ = self.records.shape
+        out = torch.empty((batch, n_heads, length, self.head_dim), dtype=self.dtype, device=self.records.device)
+        if out.numel() == 0:
+            return out
+        _hip.on_current_device(self.records)
+        _hip.check(
+            _hip.lib().rd_kv_dequantize(
+                _hip.ptr(self.records), self.strides(), self.bits, _hip.dtype_code(self.dtype), batch, n_heads, 0,
+                length, self.head_dim, length, _hip.ptr(out),
+                (ctypes.c_int64 * 3)(out.stride(0), out.stride(1), out.stride(2)), _hip.stream(),
+            )
+        )
+        return out
 
 
 class View:
@@ -36,26 +81,60 @@ class View:
     @property
     def shape(self) -> Tuple[int, int, int, int]:
         _, _, batch_size, n_heads, _, head_dim = self._cache.shape
-        return (batch_size, n_heads, self.length, head_dim)
+        return (batch_size, n_heads, self.length, head_dim if self.bits is None else self._owner.head_dim)
 
-    def cat(self, new_kv: torch.Tensor) -> torch.Tensor:
-        """Appends (batch, n_heads, n_new, head_dim) rows in place and returns rows [0, length)."""
-        _, _, batch_size, n_heads, max_length, head_dim = self._cache.shape
+    @property
+    def bits(self) -> Optional[int]:
+        """4 or 8 for a cache that holds its rows in so many bits, None for one in the model's type."""
+        return None if self._owner is None else self._owner.bits
+
+    def append(self, new_kv: torch.Tensor) -> None:
+        """Appends (batch, n_heads, n_new, head_dim) rows in place (rounded to the cache's bits)."""
+        batch_size, n_heads, _, head_dim = self.shape
+        max_length = self._cache.shape[4]
         n_new = new_kv.shape[2]
         assert new_kv.shape == (batch_size, n_heads, n_new, head_dim)
         assert self.length + n_new <= max_length
         if self._owner is not None:
             self._owner.materialize()
         slab = self._cache[self._layer, self._kv]
-        slab[:, :, self.length : self.length + n_new, :] = new_kv
+        if self.bits is None:
+            slab[:, :, self.length : self.length + n_new, :] = new_kv
+        elif new_kv.numel():
+            x = new_kv.to(self._owner.dtype)  # (what an assignment to a cache in the model's type does)
+            if x.stride(3) != 1:
+                x = x.contiguous()
+            _hip.on_current_device(x, slab)
+            _hip.check(
+                _hip.lib().rd_kv_quantize(
+                    _hip.ptr(x), (ctypes.c_int64 * 3)(x.stride(0), x.stride(1), x.stride(2)), _hip.dtype_code(x.dtype),
+                    batch_size, n_heads, n_new, head_dim, self.bits, _hip.ptr(slab),
+                    (ctypes.c_int64 * 3)(slab.stride(0), slab.stride(1), slab.stride(2)), self.length, max_length,
+                    _hip.stream(),
+                )
+            )
         self.length += n_new
-        return slab[:, :, : self.length, :]
+
+    def cat(self, new_kv: torch.Tensor) -> torch.Tensor:
+        """Appends (batch, n_heads, n_new, head_dim) rows in place and returns rows [0, length) (of a
+        cache in 4 or 8 bits: their values, read back)."""
+        self.append(new_kv)
+        return self.slice(0)
+
+    def rows(self, prev: int = 0):
+        """Rows [prev, length) as the attention reads them: a view of the cache in the model's type, or
+        the `QuantizedRows` of one in 4 or 8 bits.  With cache rows in place these are cache rows, not
+        token columns (a PreparedMask built with the cache's shifts goes with them)."""
+        rows = self._cache[self._layer, self._kv, :, :, prev : self.length, :]
+        if self.bits is None:
+            return rows
+        return QuantizedRows(rows, self.bits, self._owner.head_dim, self._owner.dtype, self._cache.shape[4] - prev)
 
     def slice(self, prev: int) -> torch.Tensor:
-        """Rows [prev, length)."""
+        """Rows [prev, length) (of a cache in 4 or 8 bits: their values, read back)."""
         if self._owner is not None:
             self._owner.materialize()
-        return self._cache[self._layer, self._kv, :, :, prev : self.length, :]
+        return self.rows(prev) if self.bits is None else self.rows(prev).read()
 
 
 def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
@@ -71,10 +150,17 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Te
 
     With `rows`, q, k and v are (total, heads*D) / (total, kv_heads*D): only the slots that exist.
     The cache still grows by n rows per batch row (the slots that do not exist keep what the
-    cache held), and q comes back as a (total, heads, D) view."""
+    cache held), and q comes back as a (total, heads, D) view.
+
+    A cache in 4 or 8 bits takes the records of the exact rotated keys and of the values, and keys and
+    values come back as its `QuantizedRows`.  q is then rotated into a tensor of its own (rounded once; the
+    projection's output is left as it was), of which the result is a view; rows behind the last token of
+    a packed batch are not written."""
     key_view, value_view = past_key_value
     cache = key_view._cache
-    _, _, batch, n_kv_heads, max_length, head_dim = cache.shape
+    bits = key_view.bits
+    batch, n_kv_heads, _, head_dim = key_view.shape
+    max_length = cache.shape[4]
     if rows is None:
         n_new = q.shape[1]
         lead = (batch, n_new)
@@ -88,7 +174,7 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Te
     assert q.shape == (*lead, n_heads * head_dim) and q.stride(-1) == 1
     assert k.shape == (*lead, n_kv_heads * head_dim) and k.stride(-1) == 1
     assert v.shape == k.shape and v.stride(-1) == 1
-    assert q.dtype == k.dtype == v.dtype == cache.dtype == cos.dtype == sin.dtype
+    assert q.dtype == k.dtype == v.dtype == (cache.dtype if bits is None else key_view._owner.dtype) == cos.dtype == sin.dtype
     assert cos.shape == sin.shape and cos.shape[1] == head_dim and cos.is_contiguous() and sin.is_contiguous()
     assert position_ids.shape == (batch, n_new) and position_ids.dtype == torch.long and position_ids.stride(1) == 1
     assert key_view.length == value_view.length and key_view.length + n_new <= max_length
@@ -97,6 +183,23 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Te
     v_slab = cache[key_view._layer, 1]
     owner = key_view._owner
     shift = owner.shift if owner is not None and owner.rows_in_place else None
+    if bits is not None:
+        _hip.on_current_device(q, k, v, cos, sin, position_ids, cache)
+        q_out = torch.empty((*lead, n_heads * head_dim), dtype=q.dtype, device=q.device)
+        _hip.check(
+            _hip.lib().rd_rope_append_quant(
+                _hip.ptr(q), strides(q), _hip.ptr(k), strides(k), _hip.ptr(v), strides(v),
+                _hip.dtype_code(q.dtype), batch, n_new, n_heads,
+                n_kv_heads, head_dim, _hip.ptr(cos), _hip.ptr(sin), cos.shape[0], _hip.ptr(position_ids),
+                position_ids.stride(0), _hip.ptr(q_out), strides(q_out), _hip.ptr(k_slab), _hip.ptr(v_slab),
+                (ctypes.c_int64 * 3)(k_slab.stride(0), k_slab.stride(1), k_slab.stride(2)), bits, key_view.length,
+                max_length, _hip.ptr(rows.row_start) if rows is not None else None, _hip.ptr(shift), _hip.stream(),
+            )
+        )
+        key_view.length += n_new
+        value_view.length += n_new
+        q_heads = q_out.unflatten(-1, (n_heads, head_dim))
+        return q_heads.transpose(1, 2) if rows is None else q_heads, key_view.rows(), value_view.rows()
     _hip.check(
         _hip.lib().rd_rope_append(
             _hip.ptr(q), strides(q), _hip.ptr(k), strides(k), _hip.ptr(v), strides(v),
@@ -126,10 +229,21 @@ class Cache:
         head_dim: int,
         dtype: torch.dtype,
         device: torch.device,
+        bits: Optional[int] = None,
     ) -> None:
+        """bits: None for rows in `dtype` (the reference's cache); 4 or 8 for rows rounded from `dtype`
+        to so many bits as they are written (head_dim a multiple of 32, at most 256)."""
+        self.bits, self.dtype, self.head_dim = bits, dtype, head_dim
+        row, element = head_dim, dtype
+        if bits is not None:
+            _hip.dtype_code(dtype)
+            row, element = _hip.lib().rd_kv_quant_row_bytes(int(bits), head_dim), torch.uint8
+            if bits not in (4, 8) or row == 0:
+                raise ValueError(f"a cache in {bits} bits with head_dim {head_dim}: bits must be 4 or 8, head_dim a "
+                                 "multiple of 32 and at most 256")
         # (the attention reads only the cache rows of keys that somebody attends to, so nothing is
         # asked of the memory around a row's live rows; zeros as upstream, kv_cache.py:49-53)
-        self._storage = torch.zeros([n_layers, 2, batch_size, n_heads, max_length, head_dim], dtype=dtype, device=device)
+        self._storage = torch.zeros([n_layers, 2, batch_size, n_heads, max_length, row], dtype=element, device=device)
         self._cache = self._storage
         self.sliced = tuple(
             (View(self._cache, layer, 0, self), View(self._cache, layer, 1, self)) for layer in range(n_layers)
@@ -152,8 +266,8 @@ class Cache:
 
     # -- geometry handed to the C ABI ---------------------------------------------------------
     def _geometry(self):
-        n_layers, _, batch, n_heads, max_len, head_dim = self._cache.shape
-        return n_layers, batch, n_heads, max_len, head_dim * self._cache.element_size()
+        n_layers, _, batch, n_heads, max_len, row = self._cache.shape  # (row: head_dim elements, or a record's bytes)
+        return n_layers, batch, n_heads, max_len, row * self._cache.element_size()
 
     def materialize(self) -> None:
         """Moves the rows to the layout in which column and cache row agree (no-op unless a

@@ -147,6 +147,9 @@ class RecurrentDrafting(torch.nn.Module):
         # True: the decode loop leaves the KV cache rows where they are when the ids are re-aligned
         # (kv_cache.Cache.rows_in_place); False: it moves them every step, as the reference does.
         self.kv_rows_in_place = True
+        # 4 or 8: the KV cache of `generate` holds its rows in so many bits (kv_cache.Cache); None: in
+        # the model's type, as the reference does.
+        self.kv_bits: Optional[int] = None
 
     def llm_n_kv_heads(self) -> int:
         if isinstance(self.llm, modeling_llama.LlamaForCausalLM):
@@ -258,6 +261,7 @@ class RecurrentDrafting(torch.nn.Module):
             head_dim=cfg.hidden_size // cfg.num_attention_heads,
             dtype=self.llm.dtype,
             device=input_ids.device,
+            bits=self.kv_bits,
         )
         context, init_tokens = _comprehend_prompt(
             self.llm, input_ids, cache, sampling_args, special_tokens.pad
