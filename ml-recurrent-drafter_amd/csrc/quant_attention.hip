@@ -189,16 +189,20 @@ struct Unit {
 };
 
 template <typename T, int BITS, int D, int RB, int WAVES>
-__global__ __launch_bounds__(WAVES * 64) void attn_quant_kernel(QuantArgs a) {
+__global__ __launch_bounds__(WAVES * 64, 2) void attn_quant_kernel(QuantArgs a) {
   using O = Ops<T>;
   using U = Unit<BITS, D, RB>;
   constexpr int kRec = record_bytes(BITS, D), kCodes = code_bytes(BITS, D);
   constexpr int kSteps = D / 32;                    // blocks of 8 dims in a K chunk
   constexpr int kCols = D / 16;                     // dims of a V column = tiles of the output
+  constexpr int kColBytes = kCols * BITS / 8;
   constexpr int kRows = 16 * RB;
   constexpr int kPitch = D + 4;                     // floats of a merged row in LDS
+  constexpr int kQPitch = D + 8;                    // 16-bit elements of a query row in LDS
+  constexpr bool kQInLds = RB > 2;
   __shared__ __attribute__((aligned(16))) float s_o[WAVES * 16 * kPitch];
   __shared__ float s_ml[WAVES * 16 * 2];
+  __shared__ __attribute__((aligned(16))) uint16_t s_q[kQInLds ? kRows * kQPitch : 8];
 
   const int hk = blockIdx.x % a.Hkv, tile = blockIdx.x / a.Hkv;
   const int b = blockIdx.y / a.max_pieces, piece = blockIdx.y % a.max_pieces;
@@ -211,70 +215,108 @@ __global__ __launch_bounds__(WAVES * 64) void attn_quant_kernel(QuantArgs a) {
   const int lo = t.begin + piece * a.piece;
   const int hi = t.hi < lo + a.piece ? t.hi : lo + a.piece;
 
-  // K and V rows of the piece's attended keys, [first, hi): what a descriptor covers
+  // K and V rows of the piece: offsets count from key lo, [first, hi) are read.  Rows from hi on read as
+  // zeros through the descriptors' range check; keys of the first unit below `first` (which nobody
+  // attends to and which may lie before the slab) read row `first` instead.
   const int shift = a.plan[RD_PLAN_HDR + 4 * b + 3];
   int first = lo > t.lo ? lo : t.lo;
   first = first > shift ? first : shift;            // (a shift is never followed out of the slab)
-  const int64_t at = (int64_t)first - shift;        // cache row of key `first`
-  int64_t n_rows = (int64_t)hi - first;
-  n_rows = n_rows < a.max_len - at ? n_rows : a.max_len - at;
-  n_rows = n_rows < 0 ? 0 : n_rows;
-  const int64_t slab = (int64_t)b * a.c_sb + (int64_t)hk * a.c_sh + (n_rows > 0 ? at * kRec : 0);
-  const int range = (int)(n_rows * kRec);
+  int64_t end = hi < a.max_len + shift ? hi : a.max_len + shift;
+  const bool any = end > first;
+  const int64_t slab = (int64_t)b * a.c_sb + (int64_t)hk * a.c_sh + ((int64_t)lo - shift) * kRec;
+  const int range = any ? (int)((end - lo) * kRec) : 0;
   const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(a.k) + slab, 0, range, 0x00020000);
   const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(a.v) + slab, 0, range, 0x00020000);
+  const int q_first = row0 / a.group;               // first query of the tile
+  const __amdgpu_buffer_rsrc_t mr = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<uint64_t*>(a.bits) + ((int64_t)b * a.n_q + q_first) * a.words, 0, 0x7fffffff, 0x00020000);
 
   // queries: B operand of the first product, lane (row l % 16, dims of chunk l / 16)
-  u32x4 qf[RB][kSteps];
-  const uint32_t* mrow[RB];
+  u32x4 qf[kQInLds ? 1 : RB][kSteps];
+  int mask_off[RB];
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb) {
     const int r = row0 + 16 * rb + col;
     const int rc = r < t.rows ? r : t.rows - 1;     // behind the last row: that row again, not written
-    const int qi = rc / a.group, h = hk * a.group + (rc - qi * a.group);
-    const T* qp = reinterpret_cast<const T*>(a.q) + t.q_off + (int64_t)h * a.q_sh + (int64_t)qi * a.q_ss + grp * (D / 4);
+    const int qi = rc / a.group;
+    mask_off[rb] = (qi - q_first) * a.words * 8;
+    if constexpr (!kQInLds) {
+      const int h = hk * a.group + (rc - qi * a.group);
+      const T* qp = reinterpret_cast<const T*>(a.q) + t.q_off + (int64_t)h * a.q_sh + (int64_t)qi * a.q_ss + grp * (D / 4);
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) qf[rb][s] = *reinterpret_cast<const u32x4*>(qp + 8 * s);
-    mrow[rb] = reinterpret_cast<const uint32_t*>(a.bits + ((int64_t)b * a.n_q + qi) * a.words);
+      for (int s = 0; s < kSteps; ++s) qf[rb][s] = *reinterpret_cast<const u32x4*>(qp + 8 * s);
+    }
   }
+  if constexpr (kQInLds) {
+    constexpr int kChunks = D / 8;
+    for (int e = tid; e < kRows * kChunks; e += WAVES * 64) {
+      const int rr = e / kChunks, c = e - rr * kChunks;
+      const int r = row0 + rr, rc = r < t.rows ? r : t.rows - 1;
+      const int qi = rc / a.group, h = hk * a.group + (rc - qi * a.group);
+      const T* qp = reinterpret_cast<const T*>(a.q) + t.q_off + (int64_t)h * a.q_sh + (int64_t)qi * a.q_ss;
+      *reinterpret_cast<u32x4*>(s_q + rr * kQPitch + 8 * c) = *reinterpret_cast<const u32x4*>(qp + 8 * c);
+    }
+    __syncthreads();
+  }
+  auto query = [&](int rb, int s) __attribute__((always_inline)) {
+    if constexpr (kQInLds) return *reinterpret_cast<const u32x4*>(s_q + (16 * rb + col) * kQPitch + grp * (D / 4) + 8 * s);
+    else return qf[rb][s];
+  };
 
   const int n_units = (hi - lo + kUnit - 1) / kUnit;
-  auto fetch = [&](U& u, int i) __attribute__((always_inline)) {
-    // (past the end: the last unit again, its loads are cheap and nobody uses them)
-    const int c = i < n_units ? i : n_units - 1;
-    const int key0 = lo + c * kUnit;
-    const int base = (key0 - first) * kRec;         // negative below `first`: out of the descriptor's range
+  // byte offsets of the lane's parts of a unit; a unit further is kUnit records further
+  const int k_lane = col * kRec + D * BITS / 32 * grp, ks_lane = col * kRec + kCodes + kSteps * grp;
+  const int v_lane = 4 * grp * kRec + kColBytes * col, vs_lane = 4 * grp * kRec + kCodes + col * kCols / kBlock;
+  // FIRST: the unit may begin below `first`
+  auto fetch_k = [&](U& u, int i, auto first_c) __attribute__((always_inline)) {
+    const int base = i * kUnit * kRec;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int off = base + (16 * h + col) * kRec;
+      int row = 16 * h * kRec;
+      if constexpr (decltype(first_c)::value) {
+        const int key = i * kUnit + 16 * h + col, least = first - lo;
+        row += key < least ? (least - key) * kRec : 0;
+      }
+      const uint32_t off = (uint32_t)(base + k_lane) + (uint32_t)row;
       if constexpr (U::kCw == 2) {
-        const u32x2 w = __builtin_amdgcn_raw_buffer_load_b64(kr, off + 8 * grp, 0, 0);
+        const u32x2 w = __builtin_amdgcn_raw_buffer_load_b64(kr, off, 0, 0);
         u.k[h][0] = w[0]; u.k[h][1] = w[1];
       } else {
 #pragma unroll
         for (int p = 0; p < U::kCw / 4; ++p) {
-          const u32x4 w = __builtin_amdgcn_raw_buffer_load_b128(kr, off + 4 * U::kCw * grp + 16 * p, 0, 0);
+          const u32x4 w = __builtin_amdgcn_raw_buffer_load_b128(kr, off + 16 * p, 0, 0);
 #pragma unroll
           for (int e = 0; e < 4; ++e) u.k[h][4 * p + e] = w[e];
         }
       }
-      if constexpr (kSteps == 4) u.ks[h] = __builtin_amdgcn_raw_buffer_load_b32(kr, off + kCodes + 4 * grp, 0, 0);
-      else u.ks[h] = __builtin_amdgcn_raw_buffer_load_b16(kr, off + kCodes + 2 * grp, 0, 0);
+      const uint32_t soff = (uint32_t)(base + ks_lane) + (uint32_t)row;
+      if constexpr (kSteps == 4) u.ks[h] = __builtin_amdgcn_raw_buffer_load_b32(kr, soff, 0, 0);
+      else u.ks[h] = __builtin_amdgcn_raw_buffer_load_b16(kr, soff, 0, 0);
     }
+  };
+  auto fetch_v = [&](U& u, int i, auto first_c) __attribute__((always_inline)) {
+    const int base = i * kUnit * kRec;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const int off = base + (16 * (j / 4) + 4 * grp + j % 4) * kRec;
-      constexpr int kColBytes = kCols * BITS / 8;
-      if constexpr (kColBytes == 2) u.v[j][0] = __builtin_amdgcn_raw_buffer_load_b16(vr, off + 2 * col, 0, 0);
-      else if constexpr (kColBytes == 4) u.v[j][0] = __builtin_amdgcn_raw_buffer_load_b32(vr, off + 4 * col, 0, 0);
+      int row = (16 * (j / 4) + j % 4) * kRec;
+      if constexpr (decltype(first_c)::value) {
+        const int key = i * kUnit + 16 * (j / 4) + 4 * grp + j % 4, least = first - lo;
+        row += key < least ? (least - key) * kRec : 0;
+      }
+      const uint32_t off = (uint32_t)(base + v_lane) + (uint32_t)row;
+      if constexpr (kColBytes == 2) u.v[j][0] = __builtin_amdgcn_raw_buffer_load_b16(vr, off, 0, 0);
+      else if constexpr (kColBytes == 4) u.v[j][0] = __builtin_amdgcn_raw_buffer_load_b32(vr, off, 0, 0);
       else {
-        const u32x2 w = __builtin_amdgcn_raw_buffer_load_b64(vr, off + 8 * col, 0, 0);
+        const u32x2 w = __builtin_amdgcn_raw_buffer_load_b64(vr, off, 0, 0);
         u.v[j][0] = w[0]; u.v[j][1] = w[1];
       }
-      u.vs[j] = __builtin_amdgcn_raw_buffer_load_b8(vr, off + kCodes + col * kCols / kBlock, 0, 0);
+      u.vs[j] = __builtin_amdgcn_raw_buffer_load_b8(vr, (uint32_t)(base + vs_lane) + (uint32_t)row, 0, 0);
     }
+  };
+  auto fetch_mask = [&](U& u, int i) __attribute__((always_inline)) {
+    const int word = lo / kUnit + (i < n_units ? i : n_units - 1);
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb) u.mask[rb] = mrow[rb][key0 / kUnit];
+    for (int rb = 0; rb < RB; ++rb) u.mask[rb] = __builtin_amdgcn_raw_buffer_load_b32(mr, mask_off[rb], 4 * word, 0);
   };
 
   f32x4 o[RB][kCols];
@@ -286,24 +328,39 @@ __global__ __launch_bounds__(WAVES * 64) void attn_quant_kernel(QuantArgs a) {
     for (int j = 0; j < kCols; ++j) o[rb][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
-  auto compute = [&](U& u) __attribute__((always_inline)) {
-    // scores: sc[rb][h] holds keys 16 h + 4 grp + i of row `col`
+  U u;
+  const int i0 = (first - lo) / kUnit + wave;       // (0 + wave, unless a shift points in front of the slab)
+  if (any && i0 < n_units) {
+    fetch_k(u, i0, std::true_type{});
+    fetch_mask(u, i0);
+    fetch_v(u, i0, std::true_type{});
+  }
+  // Each part of a unit is requested again, for the wave's next unit, as soon as it has been used: one
+  // set of registers, and the rest of the unit's work covers the trip.
+  for (int i = i0; any && i < n_units; i += WAVES) {
+    // scores: sc[rb][h] holds keys 16 h + 4 grp + e of row `col`
     f32x4 sc[RB][2];
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) sc[rb][0] = sc[rb][1] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    for (int s = 0; s < kSteps; ++s) {
+      u32x4 kf[2];
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
+      for (int h = 0; h < 2; ++h) {
         // byte s of the scales in the exponent field (the conversion looks at nothing else)
         const uint32_t e = s == 0 ? u.ks[h] << 23 : (s == 1 ? u.ks[h] << 15 : (s == 2 ? u.ks[h] << 7 : u.ks[h] >> 1));
         uint32_t w[4];
         convert<T, BITS, 4>(&u.k[h][s * BITS / 4], __uint_as_float(e), w);
-        const u32x4 kf = {w[0], w[1], w[2], w[3]};
+        kf[h] = u32x4{w[0], w[1], w[2], w[3]};
+      }
 #pragma unroll
-        for (int rb = 0; rb < RB; ++rb) sc[rb][h] = O::mfma(kf, qf[rb][s], sc[rb][h]);
+      for (int rb = 0; rb < RB; ++rb) {
+        const u32x4 qs = query(rb, s);
+        sc[rb][0] = O::mfma(kf[0], qs, sc[rb][0]);
+        sc[rb][1] = O::mfma(kf[1], qs, sc[rb][1]);
       }
     }
+    fetch_k(u, i + WAVES, std::false_type{});
     // V blocks that read back as NaN (or that no append wrote: a scale beyond the type's range)
     uint32_t worst = 0;
 #pragma unroll
@@ -332,10 +389,10 @@ __global__ __launch_bounds__(WAVES * 64) void attn_quant_kernel(QuantArgs a) {
         }
         const f32x4 count = O::mfma(bad, on, f32x4{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float poison = count[i] > 0.f ? NAN : 0.f;
+        for (int e = 0; e < 4; ++e) {
+          const float poison = count[e] > 0.f ? NAN : 0.f;
 #pragma unroll
-          for (int j = 0; j < kCols; ++j) o[rb][j][i] += poison;
+          for (int j = 0; j < kCols; ++j) o[rb][j][e] += poison;
         }
       }
     }
@@ -368,10 +425,12 @@ __global__ __launch_bounds__(WAVES * 64) void attn_quant_kernel(QuantArgs a) {
       l[rb] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
       pf[rb] = u32x4{O::pack(p[0], p[1]), O::pack(p[2], p[3]), O::pack(p[4], p[5]), O::pack(p[6], p[7])};
     }
+    fetch_mask(u, i + WAVES);
     // output tiles, two dims at a time: pairs of (dim, dim + 1) of one key -> pairs of keys of one dim
     uint32_t w[8][kCols / 2];
 #pragma unroll
     for (int j = 0; j < 8; ++j) convert<T, BITS, kCols / 2>(u.v[j], __uint_as_float(u.vs[j] << 23), w[j]);
+    fetch_v(u, i + WAVES, std::false_type{});
 #pragma unroll
     for (int d = 0; d < kCols / 2; ++d) {
       u32x4 even, odd;
@@ -385,18 +444,6 @@ __global__ __launch_bounds__(WAVES * 64) void attn_quant_kernel(QuantArgs a) {
         o[rb][2 * d] = O::mfma(even, pf[rb], o[rb][2 * d]);
         o[rb][2 * d + 1] = O::mfma(odd, pf[rb], o[rb][2 * d + 1]);
       }
-    }
-  };
-
-  if (n_rows > 0) {
-    U x, y;
-    fetch(x, wave);
-    for (int i = wave; i < n_units; i += 2 * WAVES) {
-      fetch(y, i + WAVES);
-      compute(x);
-      if (i + WAVES >= n_units) break;
-      fetch(x, i + 2 * WAVES);
-      compute(y);
     }
   }
 
@@ -619,7 +666,10 @@ struct Shape { int row_blocks, tiles, piece, max_pieces; };
 Shape shape_of(int batch, int n_heads, int n_kv_heads, int n_q, int kv_len) {
   Shape s;
   const int64_t rows = (int64_t)n_q * (n_heads / n_kv_heads);
-  s.row_blocks = rows <= 16 ? 1 : 2;
+#ifndef QRB
+#define QRB 2
+#endif
+  s.row_blocks = rows <= 16 ? 1 : (rows <= 32 ? 2 : QRB);
   s.tiles = (int)rd::ceil_div(rows, 16 * s.row_blocks);
   const int waves = s.row_blocks == 1 ? 8 : 4;
   // enough pieces that every compute unit has two workgroups, none shorter than four units per wave
@@ -643,7 +693,8 @@ void launch(const QuantArgs& a, const Shape& s, hipStream_t stream) {
   rd::ScopedTiming rd_t("attn_quant_kernel", stream);
   switch (s.row_blocks) {
     case 1: hipLaunchKernelGGL((attn_quant_kernel<T, BITS, D, 1, 8>), grid, dim3(512), 0, stream, a); break;
-    default: hipLaunchKernelGGL((attn_quant_kernel<T, BITS, D, 2, 4>), grid, dim3(256), 0, stream, a); break;
+    case 2: hipLaunchKernelGGL((attn_quant_kernel<T, BITS, D, 2, 4>), grid, dim3(256), 0, stream, a); break;
+    default: hipLaunchKernelGGL((attn_quant_kernel<T, BITS, D, 4, 4>), grid, dim3(256), 0, stream, a); break;
   }
 }
 
