@@ -65,6 +65,7 @@ struct QuantArgs {
   int B, H, Hkv, group, n_q, kv_len, words, D, bits_per_code;
   int span_blocks, max_pieces, piece;
   float scale;     // softmax scale; times log2 e for the MFMA kernel
+  float inv_scale; // its reciprocal
 };
 
 __device__ inline float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -170,10 +171,6 @@ __device__ inline float row_max(float v) {
   v = fmaxf(v, __shfl_xor(v, 16));
   return fmaxf(v, __shfl_xor(v, 32));
 }
-__device__ inline float row_sum(float v) {
-  v += __shfl_xor(v, 16);
-  return v + __shfl_xor(v, 32);
-}
 
 // ---------------------------------------------------------------------------------------------
 // MFMA kernel
@@ -188,8 +185,11 @@ struct Unit {
   uint32_t mask[RB];
 };
 
+#ifndef WPE
+#define WPE 2
+#endif
 template <typename T, int BITS, int D, int RB, int WAVES>
-__global__ __launch_bounds__(WAVES * 64, 2) void attn_quant_kernel(QuantArgs a) {
+__global__ __launch_bounds__(WAVES * 64, WPE) void attn_quant_kernel(QuantArgs a) {
   using O = Ops<T>;
   using U = Unit<BITS, D, RB>;
   constexpr int kRec = record_bytes(BITS, D), kCodes = code_bytes(BITS, D);
@@ -198,11 +198,8 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_quant_kernel(QuantArgs a) 
   constexpr int kColBytes = kCols * BITS / 8;
   constexpr int kRows = 16 * RB;
   constexpr int kPitch = D + 4;                     // floats of a merged row in LDS
-  constexpr int kQPitch = D + 8;                    // 16-bit elements of a query row in LDS
-  constexpr bool kQInLds = RB > 2;
   __shared__ __attribute__((aligned(16))) float s_o[WAVES * 16 * kPitch];
   __shared__ float s_ml[WAVES * 16 * 2];
-  __shared__ __attribute__((aligned(16))) uint16_t s_q[kQInLds ? kRows * kQPitch : 8];
 
   const int hk = blockIdx.x % a.Hkv, tile = blockIdx.x / a.Hkv;
   const int b = blockIdx.y / a.max_pieces, piece = blockIdx.y % a.max_pieces;
@@ -232,7 +229,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_quant_kernel(QuantArgs a) 
       const_cast<uint64_t*>(a.bits) + ((int64_t)b * a.n_q + q_first) * a.words, 0, 0x7fffffff, 0x00020000);
 
   // queries: B operand of the first product, lane (row l % 16, dims of chunk l / 16)
-  u32x4 qf[kQInLds ? 1 : RB][kSteps];
+  u32x4 qf[RB][kSteps];
   int mask_off[RB];
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb) {
@@ -240,44 +237,29 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_quant_kernel(QuantArgs a) 
     const int rc = r < t.rows ? r : t.rows - 1;     // behind the last row: that row again, not written
     const int qi = rc / a.group;
     mask_off[rb] = (qi - q_first) * a.words * 8;
-    if constexpr (!kQInLds) {
-      const int h = hk * a.group + (rc - qi * a.group);
-      const T* qp = reinterpret_cast<const T*>(a.q) + t.q_off + (int64_t)h * a.q_sh + (int64_t)qi * a.q_ss + grp * (D / 4);
+    const int h = hk * a.group + (rc - qi * a.group);
+    const T* qp = reinterpret_cast<const T*>(a.q) + t.q_off + (int64_t)h * a.q_sh + (int64_t)qi * a.q_ss + grp * (D / 4);
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s) qf[rb][s] = *reinterpret_cast<const u32x4*>(qp + 8 * s);
-    }
+    for (int s = 0; s < kSteps; ++s) qf[rb][s] = *reinterpret_cast<const u32x4*>(qp + 8 * s);
   }
-  if constexpr (kQInLds) {
-    constexpr int kChunks = D / 8;
-    for (int e = tid; e < kRows * kChunks; e += WAVES * 64) {
-      const int rr = e / kChunks, c = e - rr * kChunks;
-      const int r = row0 + rr, rc = r < t.rows ? r : t.rows - 1;
-      const int qi = rc / a.group, h = hk * a.group + (rc - qi * a.group);
-      const T* qp = reinterpret_cast<const T*>(a.q) + t.q_off + (int64_t)h * a.q_sh + (int64_t)qi * a.q_ss;
-      *reinterpret_cast<u32x4*>(s_q + rr * kQPitch + 8 * c) = *reinterpret_cast<const u32x4*>(qp + 8 * c);
-    }
-    __syncthreads();
-  }
-  auto query = [&](int rb, int s) __attribute__((always_inline)) {
-    if constexpr (kQInLds) return *reinterpret_cast<const u32x4*>(s_q + (16 * rb + col) * kQPitch + grp * (D / 4) + 8 * s);
-    else return qf[rb][s];
-  };
 
   const int n_units = (hi - lo + kUnit - 1) / kUnit;
-  // byte offsets of the lane's parts of a unit; a unit further is kUnit records further
-  const int k_lane = col * kRec + D * BITS / 32 * grp, ks_lane = col * kRec + kCodes + kSteps * grp;
-  const int v_lane = 4 * grp * kRec + kColBytes * col, vs_lane = 4 * grp * kRec + kCodes + col * kCols / kBlock;
-  // FIRST: the unit may begin below `first`
-  auto fetch_k = [&](U& u, int i, auto first_c) __attribute__((always_inline)) {
-    const int base = i * kUnit * kRec;
+  const int i0 = (first - lo) / kUnit + wave;       // (0 + wave, unless a shift points in front of the slab)
+  // Byte offsets of the lane's parts of unit i0.  They stay in registers and move by a unit stride per
+  // turn, so that the rows inside a unit are constants in the loads' offset fields.
+  uint32_t k_off = i0 * kUnit * kRec + col * kRec + D * BITS / 32 * grp, ks_off = i0 * kUnit * kRec + col * kRec + kCodes + kSteps * grp;
+  uint32_t v_off = i0 * kUnit * kRec + 4 * grp * kRec + kColBytes * col, vs_off = i0 * kUnit * kRec + 4 * grp * kRec + kCodes + col * kCols / kBlock;
+  constexpr uint32_t kStride = WAVES * kUnit * kRec;
+  const int least = first - lo - i0 * kUnit;        // rows of the first unit that lie below `first`, if any
+  auto fetch_k = [&](U& u, auto first_c) __attribute__((always_inline)) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      int row = 16 * h * kRec;
+      uint32_t off = k_off, soff = ks_off;
       if constexpr (decltype(first_c)::value) {
-        const int key = i * kUnit + 16 * h + col, least = first - lo;
-        row += key < least ? (least - key) * kRec : 0;
+        const int up = 16 * h + col < least ? (least - 16 * h - col) * kRec : 0;
+        off += up; soff += up;
       }
-      const uint32_t off = (uint32_t)(base + k_lane) + (uint32_t)row;
+      off += 16 * h * kRec; soff += 16 * h * kRec;
       if constexpr (U::kCw == 2) {
         const u32x2 w = __builtin_amdgcn_raw_buffer_load_b64(kr, off, 0, 0);
         u.k[h][0] = w[0]; u.k[h][1] = w[1];
@@ -289,29 +271,32 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_quant_kernel(QuantArgs a) 
           for (int e = 0; e < 4; ++e) u.k[h][4 * p + e] = w[e];
         }
       }
-      const uint32_t soff = (uint32_t)(base + ks_lane) + (uint32_t)row;
       if constexpr (kSteps == 4) u.ks[h] = __builtin_amdgcn_raw_buffer_load_b32(kr, soff, 0, 0);
       else u.ks[h] = __builtin_amdgcn_raw_buffer_load_b16(kr, soff, 0, 0);
     }
+    k_off += kStride; ks_off += kStride;
+    asm volatile("" : "+v"(k_off), "+v"(ks_off));
   };
-  auto fetch_v = [&](U& u, int i, auto first_c) __attribute__((always_inline)) {
-    const int base = i * kUnit * kRec;
+  auto fetch_v = [&](U& u, auto first_c) __attribute__((always_inline)) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      int row = (16 * (j / 4) + j % 4) * kRec;
+      uint32_t off = v_off, soff = vs_off;
+      const int row = 16 * (j / 4) + j % 4;
       if constexpr (decltype(first_c)::value) {
-        const int key = i * kUnit + 16 * (j / 4) + 4 * grp + j % 4, least = first - lo;
-        row += key < least ? (least - key) * kRec : 0;
+        const int up = row + 4 * grp < least ? (least - row - 4 * grp) * kRec : 0;
+        off += up; soff += up;
       }
-      const uint32_t off = (uint32_t)(base + v_lane) + (uint32_t)row;
+      off += row * kRec; soff += row * kRec;
       if constexpr (kColBytes == 2) u.v[j][0] = __builtin_amdgcn_raw_buffer_load_b16(vr, off, 0, 0);
       else if constexpr (kColBytes == 4) u.v[j][0] = __builtin_amdgcn_raw_buffer_load_b32(vr, off, 0, 0);
       else {
         const u32x2 w = __builtin_amdgcn_raw_buffer_load_b64(vr, off, 0, 0);
         u.v[j][0] = w[0]; u.v[j][1] = w[1];
       }
-      u.vs[j] = __builtin_amdgcn_raw_buffer_load_b8(vr, (uint32_t)(base + vs_lane) + (uint32_t)row, 0, 0);
+      u.vs[j] = __builtin_amdgcn_raw_buffer_load_b8(vr, soff, 0, 0);
     }
+    v_off += kStride; vs_off += kStride;
+    asm volatile("" : "+v"(v_off), "+v"(vs_off));
   };
   auto fetch_mask = [&](U& u, int i) __attribute__((always_inline)) {
     const int word = lo / kUnit + (i < n_units ? i : n_units - 1);
@@ -319,139 +304,154 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_quant_kernel(QuantArgs a) 
     for (int rb = 0; rb < RB; ++rb) u.mask[rb] = __builtin_amdgcn_raw_buffer_load_b32(mr, mask_off[rb], 4 * word, 0);
   };
 
-  f32x4 o[RB][kCols];
-  float m[RB], l[RB];
-#pragma unroll
-  for (int rb = 0; rb < RB; ++rb) {
-    m[rb] = -INFINITY; l[rb] = 0.f;
-#pragma unroll
-    for (int j = 0; j < kCols; ++j) o[rb][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
+  // o: output tiles, l: row sums (the product of P with ones: every element of a lane's l is its row's sum),
+  // m: running maximum in log2 units, over: the score above which it is raised
+  f32x4 o[RB][kCols], l[RB];
+  float m[RB], over[RB];
+  const u32x4 ones = {O::kOne * 0x10001u, O::kOne * 0x10001u, O::kOne * 0x10001u, O::kOne * 0x10001u};
 
-  U u;
-  const int i0 = (first - lo) / kUnit + wave;       // (0 + wave, unless a shift points in front of the slab)
-  if (any && i0 < n_units) {
-    fetch_k(u, i0, std::true_type{});
-    fetch_mask(u, i0);
-    fetch_v(u, i0, std::true_type{});
-  }
   // Each part of a unit is requested again, for the wave's next unit, as soon as it has been used: one
   // set of registers, and the rest of the unit's work covers the trip.
-  for (int i = i0; any && i < n_units; i += WAVES) {
-    // scores: sc[rb][h] holds keys 16 h + 4 grp + e of row `col`
-    f32x4 sc[RB][2];
-#pragma unroll
-    for (int rb = 0; rb < RB; ++rb) sc[rb][0] = sc[rb][1] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      u32x4 kf[2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        // byte s of the scales in the exponent field (the conversion looks at nothing else)
-        const uint32_t e = s == 0 ? u.ks[h] << 23 : (s == 1 ? u.ks[h] << 15 : (s == 2 ? u.ks[h] << 7 : u.ks[h] >> 1));
-        uint32_t w[4];
-        convert<T, BITS, 4>(&u.k[h][s * BITS / 4], __uint_as_float(e), w);
-        kf[h] = u32x4{w[0], w[1], w[2], w[3]};
-      }
-#pragma unroll
-      for (int rb = 0; rb < RB; ++rb) {
-        const u32x4 qs = query(rb, s);
-        sc[rb][0] = O::mfma(kf[0], qs, sc[rb][0]);
-        sc[rb][1] = O::mfma(kf[1], qs, sc[rb][1]);
-      }
-    }
-    fetch_k(u, i + WAVES, std::false_type{});
-    // V blocks that read back as NaN (or that no append wrote: a scale beyond the type's range)
-    uint32_t worst = 0;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) worst = u.vs[j] > worst ? u.vs[j] : worst;
-    constexpr uint32_t kCap = (uint32_t)scale_max(BITS, O::kF16);
-    if (__builtin_expect(__ballot(worst > kCap) != 0, 0)) {
-      u32x4 bad;
-#pragma unroll
-      for (int j = 0; j < 8; j += 2) {
-        bad[j / 2] = (u.vs[j] > kCap ? O::kOne : 0u) | ((u.vs[j + 1] > kCap ? O::kOne : 0u) << 16);
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const bool is_bad = u.vs[j] > kCap;
-#pragma unroll
-        for (int w = 0; w < U::kVw; ++w) u.v[j][w] = is_bad ? 0u : u.v[j][w];
-        u.vs[j] = is_bad ? 127u : u.vs[j];
-      }
-#pragma unroll
-      for (int rb = 0; rb < RB; ++rb) {
-        u32x4 on;
-#pragma unroll
-        for (int j = 0; j < 8; j += 2) {
-          const uint32_t two = u.mask[rb] >> (16 * (j / 4) + 4 * grp + j % 4);
-          on[j / 2] = ((two & 1) ? O::kOne : 0u) | ((two & 2) ? O::kOne << 16 : 0u);
-        }
-        const f32x4 count = O::mfma(bad, on, f32x4{0.f, 0.f, 0.f, 0.f});
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float poison = count[e] > 0.f ? NAN : 0.f;
-#pragma unroll
-          for (int j = 0; j < kCols; ++j) o[rb][j][e] += poison;
-        }
-      }
-    }
-    // probabilities
-    u32x4 pf[RB];
+  auto sweep = [&](auto check_c) __attribute__((always_inline)) {
+    constexpr bool kCheck = decltype(check_c)::value;
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
-      const uint32_t w = u.mask[rb];
-      float x[8];
+      m[rb] = -INFINITY; over[rb] = -INFINITY; l[rb] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = sc[rb][j / 4][j % 4];
-      if (__ballot(w != 0xffffffffu) != 0) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = ((w >> (4 * grp)) >> (16 * (j / 4) + j % 4)) & 1 ? x[j] : -INFINITY;
-      }
-      float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-      top *= a.scale;
-      if (__ballot(top > m[rb] + 8.f) != 0) {
-        const float up = fmaxf(m[rb], row_max(top));
-        const float keep = up == -INFINITY ? 1.f : fast_exp2(m[rb] - up);
-        m[rb] = up;
-        l[rb] *= keep;
-#pragma unroll
-        for (int j = 0; j < kCols; ++j) o[rb][j] *= keep;
-      }
-      const float m_use = fmaxf(m[rb], -3.4e38f);   // nothing attended yet: every p below is exp2(-inf)
-      float p[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) p[j] = fast_exp2(__builtin_fmaf(x[j], a.scale, -m_use));
-      l[rb] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
-      pf[rb] = u32x4{O::pack(p[0], p[1]), O::pack(p[2], p[3]), O::pack(p[4], p[5]), O::pack(p[6], p[7])};
+      for (int j = 0; j < kCols; ++j) o[rb][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    fetch_mask(u, i + WAVES);
-    // output tiles, two dims at a time: pairs of (dim, dim + 1) of one key -> pairs of keys of one dim
-    uint32_t w[8][kCols / 2];
+    if (!any || i0 >= n_units) return;
+    U u;
+    fetch_k(u, std::true_type{});
+    fetch_mask(u, i0);
+    fetch_v(u, std::true_type{});
+    for (int i = i0; i < n_units; i += WAVES) {
+      // scores: sc[rb][h] holds keys 16 h + 4 grp + e of row `col`
+      f32x4 sc[RB][2];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) convert<T, BITS, kCols / 2>(u.v[j], __uint_as_float(u.vs[j] << 23), w[j]);
-    fetch_v(u, i + WAVES, std::false_type{});
+      for (int rb = 0; rb < RB; ++rb) sc[rb][0] = sc[rb][1] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int d = 0; d < kCols / 2; ++d) {
-      u32x4 even, odd;
+      for (int s = 0; s < kSteps; ++s) {
+        u32x4 kf[2];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        even[j] = __builtin_amdgcn_perm(w[2 * j + 1][d], w[2 * j][d], 0x05040100u);
-        odd[j] = __builtin_amdgcn_perm(w[2 * j + 1][d], w[2 * j][d], 0x07060302u);
+        for (int h = 0; h < 2; ++h) {
+          // byte s of the scales in the exponent field (the conversion looks at nothing else)
+          const uint32_t e = s == 0 ? u.ks[h] << 23 : (s == 1 ? u.ks[h] << 15 : (s == 2 ? u.ks[h] << 7 : u.ks[h] >> 1));
+          uint32_t w[4];
+          convert<T, BITS, 4>(&u.k[h][s * BITS / 4], __uint_as_float(e), w);
+          kf[h] = u32x4{w[0], w[1], w[2], w[3]};
+        }
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
+          sc[rb][0] = O::mfma(kf[0], qf[rb][s], sc[rb][0]);
+          sc[rb][1] = O::mfma(kf[1], qf[rb][s], sc[rb][1]);
+        }
       }
+      fetch_k(u, std::false_type{});
+      if constexpr (kCheck) {
+        // V blocks that read back as NaN (or that no append wrote: a scale beyond the type's range)
+        constexpr uint32_t kCap = (uint32_t)scale_max(BITS, O::kF16);
+        u32x4 bad;
+#pragma unroll
+        for (int j = 0; j < 8; j += 2)
+          bad[j / 2] = (u.vs[j] > kCap ? O::kOne : 0u) | ((u.vs[j + 1] > kCap ? O::kOne : 0u) << 16);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const bool is_bad = u.vs[j] > kCap;
+#pragma unroll
+          for (int w = 0; w < U::kVw; ++w) u.v[j][w] = is_bad ? 0u : u.v[j][w];
+          u.vs[j] = is_bad ? 127u : u.vs[j];
+        }
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
+          u32x4 on;
+#pragma unroll
+          for (int j = 0; j < 8; j += 2) {
+            const uint32_t two = u.mask[rb] >> (16 * (j / 4) + 4 * grp + j % 4);
+            on[j / 2] = ((two & 1) ? O::kOne : 0u) | ((two & 2) ? O::kOne << 16 : 0u);
+          }
+          const f32x4 count = O::mfma(bad, on, f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float poison = count[e] > 0.f ? NAN : 0.f;
+#pragma unroll
+            for (int j = 0; j < kCols; ++j) o[rb][j][e] += poison;
+          }
+        }
+      }
+      // probabilities
+      u32x4 pf[RB];
 #pragma unroll
       for (int rb = 0; rb < RB; ++rb) {
-        o[rb][2 * d] = O::mfma(even, pf[rb], o[rb][2 * d]);
-        o[rb][2 * d + 1] = O::mfma(odd, pf[rb], o[rb][2 * d + 1]);
+        const uint32_t w = u.mask[rb];
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = sc[rb][j / 4][j % 4];
+        if (__ballot(w != 0xffffffffu) != 0) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) x[j] = ((w >> (4 * grp)) >> (16 * (j / 4) + j % 4)) & 1 ? x[j] : -INFINITY;
+        }
+        const float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+        if (__ballot(top > over[rb]) != 0) {
+          const float up = fmaxf(m[rb], row_max(top) * a.scale);
+          const float keep = up == -INFINITY ? 1.f : fast_exp2(m[rb] - up);
+          m[rb] = up;
+          over[rb] = (up + 8.f) * a.inv_scale;
+          l[rb] *= keep;
+#pragma unroll
+          for (int j = 0; j < kCols; ++j) o[rb][j] *= keep;
+        }
+        const float m_use = fmaxf(m[rb], -3.4e38f);   // nothing attended yet: every p below is exp2(-inf)
+        float p[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) p[j] = fast_exp2(__builtin_fmaf(x[j], a.scale, -m_use));
+        pf[rb] = u32x4{O::pack(p[0], p[1]), O::pack(p[2], p[3]), O::pack(p[4], p[5]), O::pack(p[6], p[7])};
+      }
+      fetch_mask(u, i + WAVES);
+      // output tiles, two dims at a time: pairs of (dim, dim + 1) of one key -> pairs of keys of one dim
+      uint32_t w[8][kCols / 2];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) convert<T, BITS, kCols / 2>(u.v[j], __uint_as_float(u.vs[j] << 23), w[j]);
+      fetch_v(u, std::false_type{});
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb) l[rb] = O::mfma(ones, pf[rb], l[rb]);
+#pragma unroll
+      for (int d = 0; d < kCols / 2; ++d) {
+        u32x4 even, odd;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          even[j] = __builtin_amdgcn_perm(w[2 * j + 1][d], w[2 * j][d], 0x05040100u);
+          odd[j] = __builtin_amdgcn_perm(w[2 * j + 1][d], w[2 * j][d], 0x07060302u);
+        }
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
+          o[rb][2 * d] = O::mfma(even, pf[rb], o[rb][2 * d]);
+          o[rb][2 * d + 1] = O::mfma(odd, pf[rb], o[rb][2 * d + 1]);
+        }
       }
     }
+  };
+  const uint32_t k_start = k_off, ks_start = ks_off, v_start = v_off, vs_start = vs_off;
+  sweep(std::false_type{});
+  // A NaN in the output comes from one that somebody attends to, or from a NaN block of V under a masked
+  // key (0 * NaN): the wave goes over its keys once more and keeps the two apart.
+  bool odd_row = false;
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+    for (int j = 0; j < kCols; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) odd_row = odd_row || o[rb][j][e] != o[rb][j][e];
+  if (__builtin_expect(__ballot(odd_row) != 0, 0)) {
+    k_off = k_start; ks_off = ks_start; v_off = v_start; vs_off = vs_start;
+    sweep(std::true_type{});
   }
 
   // merge the waves, 16 rows at a time
   constexpr int kThreads = WAVES * 64, kQuads = D / 4;
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb) {
-    const float lsum = row_sum(l[rb]);
+    const float lsum = l[rb][0];
     if (rb > 0) __syncthreads();
     float* dst = s_o + (wave * 16 + col) * kPitch + 4 * kCols * grp;
 #pragma unroll
@@ -666,10 +666,7 @@ struct Shape { int row_blocks, tiles, piece, max_pieces; };
 Shape shape_of(int batch, int n_heads, int n_kv_heads, int n_q, int kv_len) {
   Shape s;
   const int64_t rows = (int64_t)n_q * (n_heads / n_kv_heads);
-#ifndef QRB
-#define QRB 2
-#endif
-  s.row_blocks = rows <= 16 ? 1 : (rows <= 32 ? 2 : QRB);
+  s.row_blocks = rows <= 16 ? 1 : 2;
   s.tiles = (int)rd::ceil_div(rows, 16 * s.row_blocks);
   const int waves = s.row_blocks == 1 ? 8 : 4;
   // enough pieces that every compute unit has two workgroups, none shorter than four units per wave
@@ -693,8 +690,7 @@ void launch(const QuantArgs& a, const Shape& s, hipStream_t stream) {
   rd::ScopedTiming rd_t("attn_quant_kernel", stream);
   switch (s.row_blocks) {
     case 1: hipLaunchKernelGGL((attn_quant_kernel<T, BITS, D, 1, 8>), grid, dim3(512), 0, stream, a); break;
-    case 2: hipLaunchKernelGGL((attn_quant_kernel<T, BITS, D, 2, 4>), grid, dim3(256), 0, stream, a); break;
-    default: hipLaunchKernelGGL((attn_quant_kernel<T, BITS, D, 4, 4>), grid, dim3(256), 0, stream, a); break;
+    default: hipLaunchKernelGGL((attn_quant_kernel<T, BITS, D, 2, 4>), grid, dim3(256), 0, stream, a); break;
   }
 }
 
@@ -765,7 +761,7 @@ extern "C" int rd_verify_attention_quant(const void* q, const int64_t* q_strides
   a.words = (kv_len + 63) / 64; a.D = head_dim; a.bits_per_code = bits;
   a.span_blocks = (int)rd::ceil_div(n_q, kSpanQueries);
   a.max_pieces = 1; a.piece = (int)(rd::ceil_div((int64_t)kv_len + kUnit - 1, kUnit) * kUnit);
-  a.scale = scale;
+  a.scale = scale; a.inv_scale = 1.f;
   hipStream_t s = rd::as_stream(stream);
   auto whole = [](const int64_t* st, int m) { return st[0] % m == 0 && st[1] % m == 0 && st[2] % m == 0; };
   const bool mfma = !force_generic && mfma_shape(dtype, head_dim) && al(q, 16) && al(out, 8) && whole(q_strides, 8) && whole(o_strides, 4);
@@ -775,6 +771,7 @@ extern "C" int rd_verify_attention_quant(const void* q, const int64_t* q_strides
                "%s: grid too large", who);
     a.max_pieces = sh.max_pieces; a.piece = sh.piece;
     a.scale = scale * 1.4426950408889634f;
+    a.inv_scale = 1.f / a.scale;
     const int group_rows = 16 * sh.row_blocks;
     if (sh.max_pieces > 1) {
       const size_t need = rd_verify_attention_quant_workspace_bytes(dtype, batch, n_heads, n_kv_heads, n_q, kv_len, head_dim);

@@ -4,7 +4,8 @@ without), read back, moved, and attended over.
 Records and values are compared bit for bit.  Tolerance of the attention, per output element o = sum p v
 with weights p (sum 1) and A = sum p |v|, u = eps / 2 of the model's type:
   u |o|                     the output's rounding
-  u A                       every weight rounded once for the second product
+  u (A + |o|)               every weight rounded once, for the second product and for the sum it is divided by:
+                            sum p d (v - o) with |d| <= u
   2 d A                     scores off by d move numerator and denominator by a factor e^d each;
                             d = D 2^-23 scale max_k sum |q k| (fp32 sums of exact products) + |s| 2^-22
                             (the score in log2 units, rounded twice) + 2^-21 (the exponential)
@@ -179,7 +180,7 @@ def _bound(q, k, v, mask, scale, dtype, out, size):
     tiny = n * vmax * 2.0 ** -125
     if dtype == torch.float16:
         tiny = tiny + n * 2.0 ** -25 * vmax + 2.0 ** -25
-    return u * np.abs(out) + (u + 2 * d + (n + D) * 2.0 ** -24) * size + tiny
+    return 2 * u * np.abs(out) + (u + 2 * d + (n + D) * 2.0 ** -24) * size + tiny
 
 
 def _tree_mask(rng, batch, n, prev, pads):
