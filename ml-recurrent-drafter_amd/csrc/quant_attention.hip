@@ -8,11 +8,12 @@
 //   attn_quant_generic_kernel  every other type and head size the cache has
 //
 // attn_quant_kernel.  The query heads of a kv head are folded into the rows (row = query * group +
-// head in group), so that K and V are read once per kv head.  A workgroup owns 16 * RB rows and a
-// piece of the keys; its waves take the 32-key units of the piece in turn, each with a running
-// maximum, sum and accumulators of its own for all the rows, and are merged through LDS at the end.
-// No tile passes through LDS and no wave waits for another inside the loop: a wave's loads land in
-// the operand layout of the matrix instructions.
+// head in group), so that K and V are read once per kv head.  A workgroup owns 16 * RB * R rows and a
+// piece of the keys: R waves side by side take 16 * RB rows each, K waves behind each other take the 32-key
+// units of the piece in turn, each with a running maximum, sum and accumulators of its own, merged through
+// LDS at the end.  Records travel memory -> registers (whole contiguous units, 16 bytes per lane) -> LDS as
+// they lie in memory; the operands of the matrix instructions are read from there without a bank conflict
+// (rows of 48, 80 and 144 bytes spread 16 lanes over all banks), codes become 16-bit numbers in registers.
 //   S^T = K Q^T  A operand: lane (key l % 16, chunk l / 16) needs 8 consecutive k-slots per step.  The
 //                order of the dims in a dot product is free, so chunk c of the record is dims
 //                [c D/4, (c+1) D/4): D/4 contiguous codes per lane, one block of 8 per step.
@@ -53,6 +54,7 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kUnit = 32;        // keys a wave takes at a time
 constexpr int kSpanQueries = 16; // queries that share an entry of the span table
+constexpr int kSpanInts = 4;     // {first key, one past the last, full_lo, full_hi} of those queries
 
 struct QuantArgs {
   const void* q; int64_t q_sb, q_sh, q_ss;       // elements
@@ -137,6 +139,7 @@ struct Tile {
   int lo, hi;       // the tile's attended keys lie in [lo, hi)
   int begin;        // lo rounded down to a unit: pieces are counted from here
   int n_pieces;     // at least 1: piece 0 of a tile that attends to nothing writes its zeros
+  int full_lo, full_hi;  // every row attends to every key of [full_lo, full_hi): whole units, maybe none
 };
 __device__ inline Tile tile_of(const QuantArgs& a, int b, int row0, int rows_per_tile) {
   Tile t;
@@ -152,19 +155,26 @@ __device__ inline Tile tile_of(const QuantArgs& a, int b, int row0, int rows_per
   }
   t.rows = n * a.group;
   t.lo = a.kv_len; t.hi = 0;
+  t.full_lo = 0; t.full_hi = a.kv_len;
   if (row0 < t.rows) {
     const int end = row0 + rows_per_tile < t.rows ? row0 + rows_per_tile : t.rows;
     const int s0 = row0 / a.group / kSpanQueries, s1 = (end - 1) / a.group / kSpanQueries;
     for (int s = s0; s <= s1; ++s) {
-      const int32_t* sp = a.spans + 2 * ((int64_t)b * a.span_blocks + s);
+      const int32_t* sp = a.spans + kSpanInts * ((int64_t)b * a.span_blocks + s);
       t.lo = sp[0] < t.lo ? sp[0] : t.lo;
       t.hi = sp[1] > t.hi ? sp[1] : t.hi;
+      t.full_lo = sp[2] > t.full_lo ? sp[2] : t.full_lo;
+      t.full_hi = sp[3] < t.full_hi ? sp[3] : t.full_hi;
     }
   }
   t.begin = t.lo / kUnit * kUnit;
   t.n_pieces = t.hi > t.lo ? (t.hi - t.begin + a.piece - 1) / a.piece : 1;
   return t;
 }
+
+// max(a, b) as one instruction (fmaxf first quiets each operand that came out of the matrix pipeline); a NaN
+// may lose, which is fine for a running maximum: its row ends as NaN whatever the maximum
+__device__ inline float larger(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, INFINITY); }
 
 // the lanes l, l ^ 16, l ^ 32, l ^ 48 share a query row
 __device__ inline float row_max(float v) {
@@ -175,53 +185,56 @@ __device__ inline float row_max(float v) {
 // ---------------------------------------------------------------------------------------------
 // MFMA kernel
 // ---------------------------------------------------------------------------------------------
-// A unit on its way: codes and scales of 32 keys and the rows' mask bits for them.
-template <int BITS, int D, int RB>
-struct Unit {
-  static constexpr int kCw = D * BITS / 128;        // dwords of a lane's K chunk (D/4 codes)
-  static constexpr int kVw = D * BITS / 512 > 0 ? D * BITS / 512 : 1;  // dwords of a lane's V column (D/16 codes)
-  uint32_t k[2][kCw], ks[2];
-  uint32_t v[8][kVw], vs[8];
-  uint32_t mask[RB];
-};
-
-#ifndef WPE
-#define WPE 2
-#endif
-template <typename T, int BITS, int D, int RB, int WAVES>
-__global__ __launch_bounds__(WAVES * 64, WPE) void attn_quant_kernel(QuantArgs a) {
+template <typename T, int BITS, int D, int RB, int R, int K>
+__global__ __launch_bounds__(R * K * 64, 2) void attn_quant_kernel(QuantArgs a) {
   using O = Ops<T>;
-  using U = Unit<BITS, D, RB>;
   constexpr int kRec = record_bytes(BITS, D), kCodes = code_bytes(BITS, D);
   constexpr int kSteps = D / 32;                    // blocks of 8 dims in a K chunk
   constexpr int kCols = D / 16;                     // dims of a V column = tiles of the output
   constexpr int kColBytes = kCols * BITS / 8;
-  constexpr int kRows = 16 * RB;
+  constexpr int kWaves = R * K;
+  constexpr int kRows = 16 * RB * R;
   constexpr int kPitch = D + 4;                     // floats of a merged row in LDS
-  __shared__ __attribute__((aligned(16))) float s_o[WAVES * 16 * kPitch];
-  __shared__ float s_ml[WAVES * 16 * 2];
+  constexpr int kKw = D * BITS / 128;               // dwords of a lane's K chunk (D/4 codes)
+  constexpr int kVw = kColBytes > 4 ? 2 : 1;        // dwords of a lane's V column (D/16 codes)
+  constexpr int kUnitBytes = kUnit * kRec;          // the records of a unit follow each other
+  constexpr int kLoads = (kUnitBytes + 1023) / 1024;  // 16 bytes per lane each
+  constexpr int kTail = kUnitBytes / 16 - 64 * (kLoads - 1);  // lanes of the last one that read
+  constexpr int kRawBytes = kLoads * 1024;
+  // R > 1: what the waves side by side read of a unit are its operands, converted once: 2 kSteps of K, kCols of V
+  constexpr bool kShared = R > 1;
+  constexpr int kOperandBytes = kShared ? (2 * kSteps + kCols) * 1024 : 0;
+  constexpr int kMaskWords = (kRows + 63) / 64;     // mask words a lane brings for a unit: one per row of the tile
+  constexpr int kMaskAt = kOperandBytes > 2 * kRawBytes ? kOperandBytes : 2 * kRawBytes;
+  constexpr int kSlotBytes = kMaskAt + 4 * kRows;
+  // a slot per wave (records of K, then of V, or operands), later the rows they merge
+  constexpr int kMergeBytes = K > 1 ? kWaves * 16 * kPitch * 4 : 0;
+  constexpr int kLdsBytes = kWaves * kSlotBytes > kMergeBytes ? kWaves * kSlotBytes : kMergeBytes;
+  __shared__ __attribute__((aligned(16))) char s_mem[kLdsBytes];
+  __shared__ float s_ml[kWaves * 16 * 2];
+  float* const s_o = reinterpret_cast<float*>(s_mem);
 
   const int hk = blockIdx.x % a.Hkv, tile = blockIdx.x / a.Hkv;
   const int b = blockIdx.y / a.max_pieces, piece = blockIdx.y % a.max_pieces;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, grp = lane >> 4;
+  const int row_wave = wave % R, key_wave = wave / R;
   const int row0 = tile * kRows;
   const Tile t = tile_of(a, b, row0, kRows);
   if (row0 >= t.rows || piece >= t.n_pieces) return;
   const int lo = t.begin + piece * a.piece;
   const int hi = t.hi < lo + a.piece ? t.hi : lo + a.piece;
 
-  // K and V rows of the piece: offsets count from key lo, [first, hi) are read.  Rows from hi on read as
-  // zeros through the descriptors' range check; keys of the first unit below `first` (which nobody
-  // attends to and which may lie before the slab) read row `first` instead.
+  // K and V rows of the piece through descriptors that begin at key lo (or at the slab's first row, `skip`
+  // keys further, where a shift puts lo in front of it) and end behind the last attended key: rows outside
+  // read as zeros without touching memory.
   const int shift = a.plan[RD_PLAN_HDR + 4 * b + 3];
-  int first = lo > t.lo ? lo : t.lo;
-  first = first > shift ? first : shift;            // (a shift is never followed out of the slab)
-  int64_t end = hi < a.max_len + shift ? hi : a.max_len + shift;
-  const bool any = end > first;
-  const int64_t slab = (int64_t)b * a.c_sb + (int64_t)hk * a.c_sh + ((int64_t)lo - shift) * kRec;
-  const int range = any ? (int)((end - lo) * kRec) : 0;
+  const int skip = shift > lo ? shift - lo : 0;
+  const int64_t end = hi < a.max_len + shift ? hi : a.max_len + shift;
+  const bool any = end > (int64_t)lo + skip;
+  const int64_t slab = (int64_t)b * a.c_sb + (int64_t)hk * a.c_sh + (any ? ((int64_t)lo + skip - shift) * kRec : 0);
+  const int range = any ? (int)((end - lo - skip) * kRec) : 0;
   const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(a.k) + slab, 0, range, 0x00020000);
   const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(a.v) + slab, 0, range, 0x00020000);
   const int q_first = row0 / a.group;               // first query of the tile
@@ -230,79 +243,167 @@ __global__ __launch_bounds__(WAVES * 64, WPE) void attn_quant_kernel(QuantArgs a
 
   // queries: B operand of the first product, lane (row l % 16, dims of chunk l / 16)
   u32x4 qf[RB][kSteps];
-  int mask_off[RB];
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb) {
-    const int r = row0 + 16 * rb + col;
+    const int r = row0 + 16 * (RB * row_wave + rb) + col;
     const int rc = r < t.rows ? r : t.rows - 1;     // behind the last row: that row again, not written
     const int qi = rc / a.group;
-    mask_off[rb] = (qi - q_first) * a.words * 8;
     const int h = hk * a.group + (rc - qi * a.group);
     const T* qp = reinterpret_cast<const T*>(a.q) + t.q_off + (int64_t)h * a.q_sh + (int64_t)qi * a.q_ss + grp * (D / 4);
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) qf[rb][s] = *reinterpret_cast<const u32x4*>(qp + 8 * s);
   }
 
+  int mask_off[kMaskWords];                         // of the rows whose mask words the lane brings
+#pragma unroll
+  for (int x = 0; x < kMaskWords; ++x) {
+    const int r = row0 + (lane + 64 * x) % kRows;
+    mask_off[x] = ((r < t.rows ? r : t.rows - 1) / a.group - q_first) * a.words * 8;
+  }
+
   const int n_units = (hi - lo + kUnit - 1) / kUnit;
-  const int i0 = (first - lo) / kUnit + wave;       // (0 + wave, unless a shift points in front of the slab)
-  // Byte offsets of the lane's parts of unit i0.  They stay in registers and move by a unit stride per
-  // turn, so that the rows inside a unit are constants in the loads' offset fields.
-  uint32_t k_off = i0 * kUnit * kRec + col * kRec + D * BITS / 32 * grp, ks_off = i0 * kUnit * kRec + col * kRec + kCodes + kSteps * grp;
-  uint32_t v_off = i0 * kUnit * kRec + 4 * grp * kRec + kColBytes * col, vs_off = i0 * kUnit * kRec + 4 * grp * kRec + kCodes + col * kCols / kBlock;
-  constexpr uint32_t kStride = WAVES * kUnit * kRec;
-  const int least = first - lo - i0 * kUnit;        // rows of the first unit that lie below `first`, if any
-  auto fetch_k = [&](U& u, auto first_c) __attribute__((always_inline)) {
+  const int u0 = skip / kUnit;                      // (0, unless a shift points in front of the slab)
+  // A round: every wave brings one unit into LDS (slot = wave); the R waves side by side go over the R units
+  // of their key wave.  The next round's loads are in flight meanwhile.
+  constexpr uint32_t kStride = kWaves * kUnitBytes, kNowhere = 0x80000000u;  // (beyond every range)
+  uint32_t off_at, tail_at;                         // byte offsets of the lane in the coming unit, and in its last load
+  u32x4 rk[kLoads], rv[kLoads];
+  char* const slot_k = s_mem + wave * kSlotBytes;
+  char* const slot_v = slot_k + kRawBytes;
+  uint32_t mask[kMaskWords];
+  // which units every row of the tile attends to in full: no mask is read for those
+  auto is_full = [&](int i) __attribute__((always_inline)) {
+    const int key0 = lo + i * kUnit;
+    return key0 >= t.full_lo && key0 + kUnit <= t.full_hi;
+  };
+  auto fetch_mask = [&](int i) __attribute__((always_inline)) {
+    if (i < n_units && !is_full(i)) {
+#pragma unroll
+      for (int x = 0; x < kMaskWords; ++x) mask[x] = __builtin_amdgcn_raw_buffer_load_b32(mr, mask_off[x], 4 * (lo / kUnit + i), 0);
+    }
+  };
+  auto fetch = [&](int i) __attribute__((always_inline)) {
+    fetch_mask(i);
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) {
+      const uint32_t off = j + 1 < kLoads ? off_at + 1024 * j : tail_at;
+      rk[j] = __builtin_amdgcn_raw_buffer_load_b128(kr, off, 0, 0);
+    }
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) {
+      const uint32_t off = j + 1 < kLoads ? off_at + 1024 * j : tail_at;
+      rv[j] = __builtin_amdgcn_raw_buffer_load_b128(vr, off, 0, 0);
+    }
+    off_at += kStride; tail_at += kStride;
+    asm volatile("" : "+v"(off_at), "+v"(tail_at));
+  };
+  auto fetch_first = [&]() __attribute__((always_inline)) {
+    const int base = ((u0 + wave) * kUnit - skip) * kRec + 16 * lane;  // (negative for rows in front of the slab)
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) {
+      const int at = base + 1024 * j;
+      const uint32_t off = at < 0 || (j + 1 == kLoads && lane >= kTail) ? kNowhere : (uint32_t)at;
+      rk[j] = __builtin_amdgcn_raw_buffer_load_b128(kr, off, 0, 0);
+      rv[j] = __builtin_amdgcn_raw_buffer_load_b128(vr, off, 0, 0);
+    }
+    fetch_mask(u0 + wave);
+    off_at = (uint32_t)base + kStride;
+    tail_at = lane < kTail ? (uint32_t)base + 1024 * (kLoads - 1) + kStride : kNowhere;
+    asm volatile("" : "+v"(off_at), "+v"(tail_at));
+  };
+  // Between a wave's own writes and reads: LDS serves a wave's accesses in order, the compiler has to keep
+  // that order too.
+  auto own_order = [&]() __attribute__((always_inline)) {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  };
+  auto stage = [&](int i) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) *reinterpret_cast<u32x4*>(slot_k + 1024 * j + 16 * lane) = rk[j];
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) *reinterpret_cast<u32x4*>(slot_v + 1024 * j + 16 * lane) = rv[j];
+    if (i < n_units && !is_full(i)) {
+#pragma unroll
+      for (int x = 0; x < kMaskWords; ++x)
+        if (kRows % 64 == 0 || lane + 64 * x < kRows) *reinterpret_cast<uint32_t*>(slot_k + kMaskAt + 4 * (lane + 64 * x)) = mask[x];
+    }
+  };
+  // the lane's codes and scales of a unit's records, for the operands of the two products
+  struct Codes { uint32_t k[2][kKw], ks[2], v[8][kVw], vs[8]; };
+  auto k_codes = [&](const char* s_k, Codes& c) __attribute__((always_inline)) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      uint32_t off = k_off, soff = ks_off;
-      if constexpr (decltype(first_c)::value) {
-        const int up = 16 * h + col < least ? (least - 16 * h - col) * kRec : 0;
-        off += up; soff += up;
-      }
-      off += 16 * h * kRec; soff += 16 * h * kRec;
-      if constexpr (U::kCw == 2) {
-        const u32x2 w = __builtin_amdgcn_raw_buffer_load_b64(kr, off, 0, 0);
-        u.k[h][0] = w[0]; u.k[h][1] = w[1];
+      const char* rec = s_k + (16 * h + col) * kRec;
+      if constexpr (kKw == 2) {
+        const u32x2 w = *reinterpret_cast<const u32x2*>(rec + 8 * grp);
+        c.k[h][0] = w[0]; c.k[h][1] = w[1];
       } else {
 #pragma unroll
-        for (int p = 0; p < U::kCw / 4; ++p) {
-          const u32x4 w = __builtin_amdgcn_raw_buffer_load_b128(kr, off + 16 * p, 0, 0);
+        for (int p = 0; p < kKw / 4; ++p) {
+          const u32x4 w = *reinterpret_cast<const u32x4*>(rec + 4 * kKw * grp + 16 * p);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) u.k[h][4 * p + e] = w[e];
+          for (int e = 0; e < 4; ++e) c.k[h][4 * p + e] = w[e];
         }
       }
-      if constexpr (kSteps == 4) u.ks[h] = __builtin_amdgcn_raw_buffer_load_b32(kr, soff, 0, 0);
-      else u.ks[h] = __builtin_amdgcn_raw_buffer_load_b16(kr, soff, 0, 0);
+      if constexpr (kSteps == 4) c.ks[h] = *reinterpret_cast<const uint32_t*>(rec + kCodes + 4 * grp);
+      else c.ks[h] = *reinterpret_cast<const uint16_t*>(rec + kCodes + 2 * grp);
     }
-    k_off += kStride; ks_off += kStride;
-    asm volatile("" : "+v"(k_off), "+v"(ks_off));
   };
-  auto fetch_v = [&](U& u, auto first_c) __attribute__((always_inline)) {
+  auto v_codes = [&](const char* s_v, Codes& c) __attribute__((always_inline)) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      uint32_t off = v_off, soff = vs_off;
-      const int row = 16 * (j / 4) + j % 4;
-      if constexpr (decltype(first_c)::value) {
-        const int up = row + 4 * grp < least ? (least - row - 4 * grp) * kRec : 0;
-        off += up; soff += up;
-      }
-      off += row * kRec; soff += row * kRec;
-      if constexpr (kColBytes == 2) u.v[j][0] = __builtin_amdgcn_raw_buffer_load_b16(vr, off, 0, 0);
-      else if constexpr (kColBytes == 4) u.v[j][0] = __builtin_amdgcn_raw_buffer_load_b32(vr, off, 0, 0);
+      const char* rec = s_v + (16 * (j / 4) + 4 * grp + j % 4) * kRec;
+      if constexpr (kColBytes == 2) c.v[j][0] = *reinterpret_cast<const uint16_t*>(rec + 2 * col);
+      else if constexpr (kColBytes == 4) c.v[j][0] = *reinterpret_cast<const uint32_t*>(rec + 4 * col);
       else {
-        const u32x2 w = __builtin_amdgcn_raw_buffer_load_b64(vr, off, 0, 0);
-        u.v[j][0] = w[0]; u.v[j][1] = w[1];
+        const u32x2 w = *reinterpret_cast<const u32x2*>(rec + 8 * col);
+        c.v[j][0] = w[0]; c.v[j][1] = w[1];
       }
-      u.vs[j] = __builtin_amdgcn_raw_buffer_load_b8(vr, soff, 0, 0);
+      c.vs[j] = *reinterpret_cast<const uint8_t*>(rec + kCodes + col * kCols / kBlock);
     }
-    v_off += kStride; vs_off += kStride;
-    asm volatile("" : "+v"(v_off), "+v"(vs_off));
   };
-  auto fetch_mask = [&](U& u, int i) __attribute__((always_inline)) {
-    const int word = lo / kUnit + (i < n_units ? i : n_units - 1);
+  // step s of the keys 16 h + col
+  auto k_operand = [&](const Codes& c, int s, int h) __attribute__((always_inline)) {
+    // byte s of the scales in the exponent field (the conversion looks at nothing else)
+    const uint32_t e = s == 0 ? c.ks[h] << 23 : (s == 1 ? c.ks[h] << 15 : (s == 2 ? c.ks[h] << 7 : c.ks[h] >> 1));
+    uint32_t w[4];
+    convert<T, BITS, 4>(&c.k[h][s * BITS / 4], __uint_as_float(e), w);
+    return u32x4{w[0], w[1], w[2], w[3]};
+  };
+  // pairs of (dim, dim + 1) of one key -> pairs of keys of one dim: dims 2 d and 2 d + 1 of the lane's column
+  struct VPairs { uint32_t w[8][kCols / 2]; };
+  auto v_pairs = [&](const Codes& c) __attribute__((always_inline)) {
+    VPairs p;
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb) u.mask[rb] = __builtin_amdgcn_raw_buffer_load_b32(mr, mask_off[rb], 4 * word, 0);
+    for (int j = 0; j < 8; ++j) convert<T, BITS, kCols / 2>(c.v[j], __uint_as_float(c.vs[j] << 23), p.w[j]);
+    return p;
   };
+  auto v_operand = [&](const VPairs& p, int j) __attribute__((always_inline)) {
+    u32x4 r;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      r[e] = __builtin_amdgcn_perm(p.w[2 * e + 1][j / 2], p.w[2 * e][j / 2], j % 2 == 0 ? 0x05040100u : 0x07060302u);
+    return r;
+  };
+  // the wave's slot: records -> operands, in the order the lanes read them back
+  auto convert_slot = [&]() __attribute__((always_inline)) {
+    Codes c;
+    own_order();
+    k_codes(slot_k, c);
+    v_codes(slot_v, c);
+    own_order();
+    u32x4* const dst = reinterpret_cast<u32x4*>(slot_k) + lane;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      dst[64 * (2 * s)] = k_operand(c, s, 0);
+      dst[64 * (2 * s + 1)] = k_operand(c, s, 1);
+    }
+    const VPairs p = v_pairs(c);
+#pragma unroll
+    for (int j = 0; j < kCols; ++j) dst[64 * (2 * kSteps + j)] = v_operand(p, j);
+  };
+  const bool active = row0 + 16 * RB * row_wave < t.rows;  // (a wave without rows only brings and converts units)
 
   // o: output tiles, l: row sums (the product of P with ones: every element of a lane's l is its row's sum),
   // m: running maximum in log2 units, over: the score above which it is raised
@@ -310,8 +411,86 @@ __global__ __launch_bounds__(WAVES * 64, WPE) void attn_quant_kernel(QuantArgs a
   float m[RB], over[RB];
   const u32x4 ones = {O::kOne * 0x10001u, O::kOne * 0x10001u, O::kOne * 0x10001u, O::kOne * 0x10001u};
 
-  // Each part of a unit is requested again, for the wave's next unit, as soon as it has been used: one
-  // set of registers, and the rest of the unit's work covers the trip.
+  // mask bits of the wave's rows for the unit whose records lie at `here`
+  auto read_mask = [&](const char* here, bool full, uint32_t (&on)[RB]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+      on[rb] = 0xffffffffu;
+      if (!full) on[rb] = *reinterpret_cast<const uint32_t*>(here + kMaskAt + 4 * (16 * (RB * row_wave + rb) + col));
+    }
+  };
+  // V of keys that no row of the wave attends to is left out, whatever it holds; blocks that read back as NaN
+  // (or that no append wrote: a scale beyond the type's range) are left out too, and rows that attend to
+  // one get their NaN from the product of the mask with the marks of those blocks.
+  auto part_nan = [&](Codes& c, const uint32_t (&on)[RB]) __attribute__((always_inline)) {
+    constexpr uint32_t kCap = (uint32_t)scale_max(BITS, O::kF16);
+    uint32_t seen = 0;
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) seen |= on[rb];
+#pragma unroll
+    for (int x = 1; x < 16; x *= 2) seen |= (uint32_t)__shfl_xor((int)seen, x);
+    u32x4 bad;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const bool unseen = ((seen >> (16 * (j / 4) + 4 * grp + j % 4)) & 1) == 0, is_bad = c.vs[j] > kCap;
+#pragma unroll
+      for (int w = 0; w < kVw; ++w) c.v[j][w] = unseen || is_bad ? 0u : c.v[j][w];
+      c.vs[j] = unseen || is_bad ? 127u : c.vs[j];
+      const uint32_t mark = is_bad && !unseen ? O::kOne : 0u;
+      if (j % 2 == 0) bad[j / 2] = mark; else bad[j / 2] |= mark << 16;
+    }
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+      u32x4 has;
+#pragma unroll
+      for (int j = 0; j < 8; j += 2) {
+        const uint32_t two = on[rb] >> (16 * (j / 4) + 4 * grp + j % 4);
+        has[j / 2] = ((two & 1) ? O::kOne : 0u) | ((two & 2) ? O::kOne << 16 : 0u);
+      }
+      const f32x4 count = O::mfma(bad, has, f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float poison = count[e] > 0.f ? NAN : 0.f;
+#pragma unroll
+        for (int j = 0; j < kCols; ++j) o[rb][j][e] += poison;
+      }
+    }
+  };
+  // Scores to weights.  sc[rb][h] holds keys 16 h + 4 grp + e of row `col`; the weights come out in the order
+  // of the second product's B operand.
+  auto weights = [&](f32x4 (&sc)[RB][2], bool full, const uint32_t (&on)[RB], u32x4 (&pf)[RB]) __attribute__((always_inline)) {
+    if (!full) {
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb) {
+        uint32_t w = on[rb] >> (4 * grp);
+        asm volatile("" : "+v"(w));                 // (keeps this a branch: as selects on every unit it would cost 24 instructions per row block)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sc[rb][j / 4][j % 4] = (w >> (16 * (j / 4) + j % 4)) & 1 ? sc[rb][j / 4][j % 4] : -INFINITY;
+      }
+    }
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+      float x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = sc[rb][j / 4][j % 4];
+      const float top = fmaxf(fmaxf(larger(x[0], x[1]), larger(x[2], x[3])), fmaxf(larger(x[4], x[5]), larger(x[6], x[7])));
+      if (__ballot(top > over[rb]) != 0) {
+        const float up = fmaxf(m[rb], row_max(top) * a.scale);
+        const float keep = up == -INFINITY ? 1.f : fast_exp2(m[rb] - up);
+        m[rb] = up;
+        over[rb] = (up + 8.f) * a.inv_scale;
+        l[rb] *= keep;
+#pragma unroll
+        for (int j = 0; j < kCols; ++j) o[rb][j] *= keep;
+      }
+      const float m_use = fmaxf(m[rb], -3.4e38f);   // nothing attended yet: every p below is exp2(-inf)
+      float p[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) p[j] = fast_exp2(__builtin_fmaf(x[j], a.scale, -m_use));
+      pf[rb] = u32x4{O::pack(p[0], p[1]), O::pack(p[2], p[3]), O::pack(p[4], p[5]), O::pack(p[6], p[7])};
+    }
+  };
+
   auto sweep = [&](auto check_c) __attribute__((always_inline)) {
     constexpr bool kCheck = decltype(check_c)::value;
 #pragma unroll
@@ -320,118 +499,122 @@ __global__ __launch_bounds__(WAVES * 64, WPE) void attn_quant_kernel(QuantArgs a
 #pragma unroll
       for (int j = 0; j < kCols; ++j) o[rb][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    if (!any || i0 >= n_units) return;
-    U u;
-    fetch_k(u, std::true_type{});
-    fetch_mask(u, i0);
-    fetch_v(u, std::true_type{});
-    for (int i = i0; i < n_units; i += WAVES) {
-      // scores: sc[rb][h] holds keys 16 h + 4 grp + e of row `col`
-      f32x4 sc[RB][2];
+    if (!any) return;                               // (uniform over the workgroup)
+    fetch_first();
+    if constexpr (!kShared) {
+      // Every wave by itself.  While unit i is multiplied with V, unit i + kWaves goes to LDS and its K codes
+      // come back, and unit i + 2 kWaves is on its way from memory.
+      int i = u0 + wave;
+      Codes c;
+      auto next = [&](int n) __attribute__((always_inline)) {
+        own_order();
+        stage(n);
+        if (n + kWaves < n_units) fetch(n + kWaves);
+        own_order();
+        k_codes(slot_k, c);
+      };
+      if (i < n_units) next(i);
+      for (; i < n_units; i += kWaves) {
+        const bool full = is_full(i);
+        uint32_t on[RB];
+        read_mask(slot_k, full, on);
+        v_codes(slot_v, c);
+        f32x4 sc[RB][2];
 #pragma unroll
-      for (int rb = 0; rb < RB; ++rb) sc[rb][0] = sc[rb][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int rb = 0; rb < RB; ++rb) sc[rb][0] = sc[rb][1] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
-        u32x4 kf[2];
+        for (int s = 0; s < kSteps; ++s) {
+          const u32x4 k0 = k_operand(c, s, 0), k1 = k_operand(c, s, 1);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          // byte s of the scales in the exponent field (the conversion looks at nothing else)
-          const uint32_t e = s == 0 ? u.ks[h] << 23 : (s == 1 ? u.ks[h] << 15 : (s == 2 ? u.ks[h] << 7 : u.ks[h] >> 1));
-          uint32_t w[4];
-          convert<T, BITS, 4>(&u.k[h][s * BITS / 4], __uint_as_float(e), w);
-          kf[h] = u32x4{w[0], w[1], w[2], w[3]};
-        }
-#pragma unroll
-        for (int rb = 0; rb < RB; ++rb) {
-          sc[rb][0] = O::mfma(kf[0], qf[rb][s], sc[rb][0]);
-          sc[rb][1] = O::mfma(kf[1], qf[rb][s], sc[rb][1]);
-        }
-      }
-      fetch_k(u, std::false_type{});
-      if constexpr (kCheck) {
-        // V blocks that read back as NaN (or that no append wrote: a scale beyond the type's range)
-        constexpr uint32_t kCap = (uint32_t)scale_max(BITS, O::kF16);
-        u32x4 bad;
-#pragma unroll
-        for (int j = 0; j < 8; j += 2)
-          bad[j / 2] = (u.vs[j] > kCap ? O::kOne : 0u) | ((u.vs[j + 1] > kCap ? O::kOne : 0u) << 16);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const bool is_bad = u.vs[j] > kCap;
-#pragma unroll
-          for (int w = 0; w < U::kVw; ++w) u.v[j][w] = is_bad ? 0u : u.v[j][w];
-          u.vs[j] = is_bad ? 127u : u.vs[j];
-        }
-#pragma unroll
-        for (int rb = 0; rb < RB; ++rb) {
-          u32x4 on;
-#pragma unroll
-          for (int j = 0; j < 8; j += 2) {
-            const uint32_t two = u.mask[rb] >> (16 * (j / 4) + 4 * grp + j % 4);
-            on[j / 2] = ((two & 1) ? O::kOne : 0u) | ((two & 2) ? O::kOne << 16 : 0u);
-          }
-          const f32x4 count = O::mfma(bad, on, f32x4{0.f, 0.f, 0.f, 0.f});
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float poison = count[e] > 0.f ? NAN : 0.f;
-#pragma unroll
-            for (int j = 0; j < kCols; ++j) o[rb][j][e] += poison;
+          for (int rb = 0; rb < RB; ++rb) {
+            sc[rb][0] = O::mfma(k0, qf[rb][s], sc[rb][0]);
+            sc[rb][1] = O::mfma(k1, qf[rb][s], sc[rb][1]);
           }
         }
+        if constexpr (kCheck) part_nan(c, on);
+        u32x4 pf[RB];
+        weights(sc, full, on, pf);
+        const VPairs pairs = v_pairs(c);
+        if (i + kWaves < n_units) next(i + kWaves);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) l[rb] = O::mfma(ones, pf[rb], l[rb]);
+#pragma unroll
+        for (int j = 0; j < kCols; ++j) {
+          const u32x4 vf = v_operand(pairs, j);
+#pragma unroll
+          for (int rb = 0; rb < RB; ++rb) o[rb][j] = O::mfma(vf, pf[rb], o[rb][j]);
+        }
       }
-      // probabilities
-      u32x4 pf[RB];
+    } else {
+      // Rounds: every wave brings and converts one unit (slot = wave), then the R waves side by side go over
+      // the R units of their key wave.
+      for (int round = u0; round < n_units; round += kWaves) {
+        __syncthreads();
+        stage(round + wave);
+        if (round + kWaves < n_units) fetch(round + kWaves + wave);
+        if constexpr (!kCheck) convert_slot();
+        __syncthreads();
+        const int last = n_units - round < key_wave * R + R ? n_units - round : key_wave * R + R;
+        u32x4 kf[2 * kSteps];                       // K operands, requested one unit ahead
+        if constexpr (!kCheck) {
 #pragma unroll
-      for (int rb = 0; rb < RB; ++rb) {
-        const uint32_t w = u.mask[rb];
-        float x[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = sc[rb][j / 4][j % 4];
-        if (__ballot(w != 0xffffffffu) != 0) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) x[j] = ((w >> (4 * grp)) >> (16 * (j / 4) + j % 4)) & 1 ? x[j] : -INFINITY;
+          for (int f = 0; f < 2 * kSteps; ++f) kf[f] = reinterpret_cast<const u32x4*>(s_mem + key_wave * R * kSlotBytes)[64 * f + lane];
         }
-        const float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-        if (__ballot(top > over[rb]) != 0) {
-          const float up = fmaxf(m[rb], row_max(top) * a.scale);
-          const float keep = up == -INFINITY ? 1.f : fast_exp2(m[rb] - up);
-          m[rb] = up;
-          over[rb] = (up + 8.f) * a.inv_scale;
-          l[rb] *= keep;
+        if (!active) continue;
+        for (int slot = key_wave * R; slot < last; ++slot) {
+          const bool full = is_full(round + slot);
+          const char* const here = s_mem + slot * kSlotBytes;
+          uint32_t on[RB];
+          read_mask(here, full, on);
+          Codes c;
+          if constexpr (kCheck) {
+            k_codes(here, c);
+            v_codes(here + kRawBytes, c);
+          }
+          f32x4 sc[RB][2];
 #pragma unroll
-          for (int j = 0; j < kCols; ++j) o[rb][j] *= keep;
-        }
-        const float m_use = fmaxf(m[rb], -3.4e38f);   // nothing attended yet: every p below is exp2(-inf)
-        float p[8];
+          for (int rb = 0; rb < RB; ++rb) sc[rb][0] = sc[rb][1] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int j = 0; j < 8; ++j) p[j] = fast_exp2(__builtin_fmaf(x[j], a.scale, -m_use));
-        pf[rb] = u32x4{O::pack(p[0], p[1]), O::pack(p[2], p[3]), O::pack(p[4], p[5]), O::pack(p[6], p[7])};
-      }
-      fetch_mask(u, i + WAVES);
-      // output tiles, two dims at a time: pairs of (dim, dim + 1) of one key -> pairs of keys of one dim
-      uint32_t w[8][kCols / 2];
+          for (int s = 0; s < kSteps; ++s) {
+            if constexpr (kCheck) {
+              kf[2 * s] = k_operand(c, s, 0);
+              kf[2 * s + 1] = k_operand(c, s, 1);
+            }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) convert<T, BITS, kCols / 2>(u.v[j], __uint_as_float(u.vs[j] << 23), w[j]);
-      fetch_v(u, std::false_type{});
+            for (int rb = 0; rb < RB; ++rb) {
+              sc[rb][0] = O::mfma(kf[2 * s], qf[rb][s], sc[rb][0]);
+              sc[rb][1] = O::mfma(kf[2 * s + 1], qf[rb][s], sc[rb][1]);
+            }
+          }
+          u32x4 vf[kCols];
+          if constexpr (!kCheck) {
+            const u32x4* const ready = reinterpret_cast<const u32x4*>(here) + lane;
 #pragma unroll
-      for (int rb = 0; rb < RB; ++rb) l[rb] = O::mfma(ones, pf[rb], l[rb]);
+            for (int j = 0; j < kCols; ++j) vf[j] = ready[64 * (2 * kSteps + j)];
+            const u32x4* const next = reinterpret_cast<const u32x4*>(s_mem + (slot + 1 < last ? slot + 1 : slot) * kSlotBytes) + lane;
 #pragma unroll
-      for (int d = 0; d < kCols / 2; ++d) {
-        u32x4 even, odd;
+            for (int f = 0; f < 2 * kSteps; ++f) kf[f] = next[64 * f];
+            __builtin_amdgcn_sched_barrier(0);      // (requested here, so that the softmax covers the way)
+          } else {
+            part_nan(c, on);
+          }
+          u32x4 pf[RB];
+          weights(sc, full, on, pf);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          even[j] = __builtin_amdgcn_perm(w[2 * j + 1][d], w[2 * j][d], 0x05040100u);
-          odd[j] = __builtin_amdgcn_perm(w[2 * j + 1][d], w[2 * j][d], 0x07060302u);
-        }
+          for (int rb = 0; rb < RB; ++rb) l[rb] = O::mfma(ones, pf[rb], l[rb]);
+          VPairs pairs;
+          if constexpr (kCheck) pairs = v_pairs(c);
 #pragma unroll
-        for (int rb = 0; rb < RB; ++rb) {
-          o[rb][2 * d] = O::mfma(even, pf[rb], o[rb][2 * d]);
-          o[rb][2 * d + 1] = O::mfma(odd, pf[rb], o[rb][2 * d + 1]);
+          for (int j = 0; j < kCols; ++j) {
+            if constexpr (kCheck) vf[j] = v_operand(pairs, j);
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb) o[rb][j] = O::mfma(vf[j], pf[rb], o[rb][j]);
+          }
         }
       }
     }
   };
-  const uint32_t k_start = k_off, ks_start = ks_off, v_start = v_off, vs_start = vs_off;
   sweep(std::false_type{});
   // A NaN in the output comes from one that somebody attends to, or from a NaN block of V under a masked
   // key (0 * NaN): the wave goes over its keys once more and keeps the two apart.
@@ -442,88 +625,125 @@ __global__ __launch_bounds__(WAVES * 64, WPE) void attn_quant_kernel(QuantArgs a
     for (int j = 0; j < kCols; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e) odd_row = odd_row || o[rb][j][e] != o[rb][j][e];
-  if (__builtin_expect(__ballot(odd_row) != 0, 0)) {
-    k_off = k_start; ks_off = ks_start; v_off = v_start; vs_off = vs_start;
-    sweep(std::true_type{});
-  }
+  if constexpr (R > 1) odd_row = __syncthreads_or(odd_row);  // (all of them: the rounds have barriers)
+  if (__builtin_expect(__ballot(odd_row) != 0, 0)) sweep(std::true_type{});
 
-  // merge the waves, 16 rows at a time
-  constexpr int kThreads = WAVES * 64, kQuads = D / 4;
-#pragma unroll
-  for (int rb = 0; rb < RB; ++rb) {
-    const float lsum = l[rb][0];
-    if (rb > 0) __syncthreads();
-    float* dst = s_o + (wave * 16 + col) * kPitch + 4 * kCols * grp;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-#pragma unroll
-      for (int j = 0; j < kCols; j += 4)
-        *reinterpret_cast<f32x4*>(dst + kCols * i + j) = f32x4{o[rb][j][i], o[rb][j + 1][i], o[rb][j + 2][i], o[rb][j + 3][i]};
+  // four neighbouring dims of row r: the result, or this piece's part of it (m in log2 units)
+  auto put = [&](int r, int dq, f32x4 acc, float top, float sum) __attribute__((always_inline)) {
+    if (t.n_pieces > 1) {
+      const int64_t slot = ((int64_t)b * a.Hkv + hk) * a.max_pieces + piece;
+      const int64_t pr = slot * ((int64_t)a.n_q * a.group) + r;
+      *reinterpret_cast<f32x4*>(a.part_o + pr * D + dq) = acc;
+      if (dq == 0) { a.part_ml[2 * pr] = top; a.part_ml[2 * pr + 1] = sum; }
+    } else {
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;  // (a NaN sum stays one)
+      const int qi = r / a.group, h = hk * a.group + (r - qi * a.group);
+      T* op = reinterpret_cast<T*>(a.out) + t.o_off + (int64_t)h * a.o_sh + (int64_t)qi * a.o_ss + dq;
+      const u32x2 w = {O::pack(acc[0] * inv, acc[1] * inv), O::pack(acc[2] * inv, acc[3] * inv)};
+      *reinterpret_cast<u32x2*>(op) = w;
     }
-    if (grp == 0) { s_ml[(wave * 16 + col) * 2] = m[rb]; s_ml[(wave * 16 + col) * 2 + 1] = lsum; }
-    __syncthreads();
-    for (int e = tid; e < 16 * kQuads; e += kThreads) {
-      const int rr = e / kQuads, dq = (e - rr * kQuads) * 4;
-      const int r = row0 + 16 * rb + rr;
+  };
+  if constexpr (K == 1) {
+    // a lane holds the dims [4 kCols grp, 4 kCols (grp + 1)) of its rows
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+      const int r = row0 + 16 * (RB * row_wave + rb) + col;
       if (r >= t.rows) continue;
-      float top = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < WAVES; ++w) top = fmaxf(top, s_ml[(w * 16 + rr) * 2]);
-      const float m_use = fmaxf(top, -3.4e38f);
-      float sum = 0.f;
-      f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+      for (int i = 0; i < 4; ++i) {
 #pragma unroll
-      for (int w = 0; w < WAVES; ++w) {
-        const float f = fast_exp2(s_ml[(w * 16 + rr) * 2] - m_use);  // a wave without keys: exp2(-inf)
-        sum += f * s_ml[(w * 16 + rr) * 2 + 1];
-        acc += f * *reinterpret_cast<const f32x4*>(s_o + (w * 16 + rr) * kPitch + dq);
+        for (int j = 0; j < kCols; j += 4)
+          put(r, 4 * kCols * grp + kCols * i + j, f32x4{o[rb][j][i], o[rb][j + 1][i], o[rb][j + 2][i], o[rb][j + 3][i]}, m[rb], l[rb][0]);
       }
-      if (t.n_pieces > 1) {
-        const int64_t slot = ((int64_t)b * a.Hkv + hk) * a.max_pieces + piece;
-        const int64_t pr = slot * ((int64_t)a.n_q * a.group) + r;
-        *reinterpret_cast<f32x4*>(a.part_o + pr * D + dq) = acc;
-        if (dq == 0) { a.part_ml[2 * pr] = top; a.part_ml[2 * pr + 1] = sum; }
-      } else {
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;  // (a NaN sum stays one)
-        const int qi = r / a.group, h = hk * a.group + (r - qi * a.group);
-        T* op = reinterpret_cast<T*>(a.out) + t.o_off + (int64_t)h * a.o_sh + (int64_t)qi * a.o_ss + dq;
-        const u32x2 w = {O::pack(acc[0] * inv, acc[1] * inv), O::pack(acc[2] * inv, acc[3] * inv)};
-        *reinterpret_cast<u32x2*>(op) = w;
+    }
+  } else {
+    // merge the K waves behind each other, 16 rows of every row wave at a time
+    constexpr int kThreads = kWaves * 64, kQuads = D / 4;
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+      __syncthreads();                              // (the units, or the rows before, are no longer read)
+      float* dst = s_o + (wave * 16 + col) * kPitch + 4 * kCols * grp;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int j = 0; j < kCols; j += 4)
+          *reinterpret_cast<f32x4*>(dst + kCols * i + j) = f32x4{o[rb][j][i], o[rb][j + 1][i], o[rb][j + 2][i], o[rb][j + 3][i]};
+      }
+      if (grp == 0) { s_ml[(wave * 16 + col) * 2] = m[rb]; s_ml[(wave * 16 + col) * 2 + 1] = l[rb][0]; }
+      __syncthreads();
+      for (int e = tid; e < 16 * R * kQuads; e += kThreads) {
+        const int rr = e / kQuads, dq = (e - rr * kQuads) * 4;  // rr: row wave * 16 + row
+        const int rw = rr / 16, r = row0 + 16 * (RB * rw + rb) + rr % 16;
+        if (r >= t.rows) continue;
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < K; ++w) top = fmaxf(top, s_ml[((w * R) * 16 + rr) * 2]);
+        const float m_use = fmaxf(top, -3.4e38f);
+        float sum = 0.f;
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < K; ++w) {
+          const int at = w * R * 16 + rr;
+          const float f = fast_exp2(s_ml[at * 2] - m_use);  // a wave without keys: exp2(-inf)
+          sum += f * s_ml[at * 2 + 1];
+          acc += f * *reinterpret_cast<const f32x4*>(s_o + at * kPitch + dq);
+        }
+        put(r, dq, acc, top, sum);
       }
     }
   }
 }
 
-// Joins the pieces of rows whose keys were cut: one thread per four dims of a row, pieces in order.
-constexpr int kMergeThreads = 256;
+// Joins the pieces of rows whose keys were cut.  D / 4 threads carry a row's dims; with many pieces `parts`
+// such groups of a workgroup share a row (piece p goes to group p % parts) and are joined through LDS.  Four
+// pieces are requested at a time: the kernel is the latency of its loads.
+constexpr int kMergeThreads = 256, kMergeMaxParts = 8;
+struct Partial { float m, l; f32x4 o; };
+__device__ inline Partial join(const Partial& a, const Partial& b) {
+  const float up = fmaxf(a.m, b.m), m_use = fmaxf(up, -3.4e38f);
+  const float fa = fast_exp2(a.m - m_use), fb = fast_exp2(b.m - m_use);
+  return {up, fa * a.l + fb * b.l, fa * a.o + fb * b.o};
+}
 template <typename T>
-__global__ __launch_bounds__(kMergeThreads) void attn_quant_merge_kernel(QuantArgs a, int rows_per_tile) {
+__global__ __launch_bounds__(kMergeThreads) void attn_quant_merge_kernel(QuantArgs a, int rows_per_tile, int parts) {
   using O = Ops<T>;
+  __shared__ Partial s_part[kMergeThreads];
   const int hk = blockIdx.y, b = blockIdx.z;
-  const int quads = a.D / 4;
-  const int64_t e = (int64_t)blockIdx.x * kMergeThreads + threadIdx.x;
-  const int64_t r64 = e / quads;
-  const int dq = (int)(e - r64 * quads) * 4;
-  if (r64 >= (int64_t)a.n_q * a.group) return;
-  const int r = (int)r64;
+  const int quads = a.D / 4, per_row = quads * parts, rows_per_wg = kMergeThreads / per_row;
+  const int sub = threadIdx.x / per_row, part = threadIdx.x % per_row / quads, dq = threadIdx.x % quads * 4;
+  const int64_t r64 = (int64_t)blockIdx.x * rows_per_wg + sub;
+  const int64_t all_rows = (int64_t)a.n_q * a.group;
+  const int r = r64 < all_rows ? (int)r64 : (int)all_rows - 1;
   const Tile t = tile_of(a, b, r / rows_per_tile * rows_per_tile, rows_per_tile);
-  if (r >= t.rows || t.n_pieces == 1) return;
-  float top = -INFINITY, sum = 0.f;
-  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  for (int p = 0; p < t.n_pieces; ++p) {
-    const int64_t pr = (((int64_t)b * a.Hkv + hk) * a.max_pieces + p) * ((int64_t)a.n_q * a.group) + r;
-    const float m = a.part_ml[2 * pr], l = a.part_ml[2 * pr + 1];
-    const f32x4 o = *reinterpret_cast<const f32x4*>(a.part_o + pr * a.D + dq);
-    const float up = fmaxf(top, m), m_use = fmaxf(up, -3.4e38f);
-    const float f0 = fast_exp2(top - m_use), f1 = fast_exp2(m - m_use);
-    sum = f0 * sum + f1 * l;
-    acc = f0 * acc + f1 * o;
-    top = up;
+  const bool mine = r64 < all_rows && r < t.rows && t.n_pieces > 1;
+  const int n = mine ? t.n_pieces : 0;
+  Partial acc = {-INFINITY, 0.f, {0.f, 0.f, 0.f, 0.f}};
+  const int64_t first = ((int64_t)b * a.Hkv + hk) * a.max_pieces;
+  for (int p0 = part; p0 < n; p0 += 4 * parts) {
+    Partial x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int p = p0 + i * parts < n ? p0 + i * parts : p0;  // (past the last piece: one that is there, not counted)
+      const int64_t pr = (first + p) * all_rows + r;
+      x[i].m = a.part_ml[2 * pr];
+      x[i].l = a.part_ml[2 * pr + 1];
+      x[i].o = *reinterpret_cast<const f32x4*>(a.part_o + pr * a.D + dq);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (p0 + i * parts < n) acc = join(acc, x[i]);
   }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  if (parts > 1) {
+    s_part[threadIdx.x] = acc;
+    __syncthreads();
+    if (part == 0)
+      for (int i = 1; i < parts; ++i) acc = join(acc, s_part[threadIdx.x + i * quads]);
+  }
+  if (!mine || part != 0) return;
+  const float inv = acc.l == 0.f ? 0.f : 1.f / acc.l;
   const int qi = r / a.group, h = hk * a.group + (r - qi * a.group);
   T* op = reinterpret_cast<T*>(a.out) + t.o_off + (int64_t)h * a.o_sh + (int64_t)qi * a.o_ss + dq;
-  const u32x2 w = {O::pack(acc[0] * inv, acc[1] * inv), O::pack(acc[2] * inv, acc[3] * inv)};
+  const u32x2 w = {O::pack(acc.o[0] * inv, acc.o[1] * inv), O::pack(acc.o[2] * inv, acc.o[3] * inv)};
   *reinterpret_cast<u32x2*>(op) = w;
 }
 
@@ -622,37 +842,88 @@ __global__ __launch_bounds__(kGenThreads) void attn_quant_generic_kernel(QuantAr
 // ---------------------------------------------------------------------------------------------
 // Span table: first and one past the last key that 16 consecutive queries of a batch row attend to.
 // ---------------------------------------------------------------------------------------------
-constexpr int kSpanThreads = 256;
+// Within it, a run of whole units that all of them attend to in full: from the first such unit to the
+// first one behind it that is not (looked for among the first 2^15 units).  A unit's words of the queries are
+// read by as many neighbouring lanes.
+constexpr int kSpanThreads = 256, kSpanBits = 1 << 15;
 __global__ __launch_bounds__(kSpanThreads) void attn_spans_kernel(const uint64_t* __restrict__ bits, int n_q, int words,
                                                                   int kv_len, int32_t* __restrict__ spans) {
-  __shared__ int s_lo[kSpanThreads / 64], s_hi[kSpanThreads / 64];
-  const int b = blockIdx.y, q0 = blockIdx.x * kSpanQueries;
+  __shared__ uint32_t s_full[kSpanBits / 32];
+  __shared__ int s_tmp[3][kSpanThreads / 64];
+  const int b = blockIdx.y, q0 = blockIdx.x * kSpanQueries, tid = threadIdx.x;
   const int nq = n_q - q0 < kSpanQueries ? n_q - q0 : kSpanQueries;
-  const uint64_t* w = bits + ((int64_t)b * n_q + q0) * words;
-  int lo = kv_len, hi = 0;
-  for (int64_t i = threadIdx.x; i < (int64_t)nq * words; i += kSpanThreads) {
-    const uint64_t x = w[i];
-    if (x == 0) continue;
-    const int key0 = (int)(i % words) * 64;
-    const int f = key0 + __ffsll((unsigned long long)x) - 1, e = key0 + 64 - __clzll((long long)x);
-    lo = f < lo ? f : lo;
-    hi = e > hi ? e : hi;
-  }
-  for (int off = 32; off > 0; off >>= 1) {
-    const int l2 = __shfl_xor(lo, off), h2 = __shfl_xor(hi, off);
-    lo = l2 < lo ? l2 : lo;
-    hi = h2 > hi ? h2 : hi;
-  }
-  if ((threadIdx.x & 63) == 0) { s_lo[threadIdx.x >> 6] = lo; s_hi[threadIdx.x >> 6] = hi; }
+  const uint32_t* rows = reinterpret_cast<const uint32_t*>(bits + ((int64_t)b * n_q + q0) * words);
+  const int units = 2 * words, full_words = ((units < kSpanBits ? units : kSpanBits) + 31) / 32;
+  for (int i = tid; i < full_words; i += kSpanThreads) s_full[i] = 0;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int i = 1; i < kSpanThreads / 64; ++i) {
-      lo = s_lo[i] < lo ? s_lo[i] : lo;
-      hi = s_hi[i] > hi ? s_hi[i] : hi;
+  int lanes = 1;                                    // per unit: a power of two
+  while (lanes < nq) lanes *= 2;
+  const int q = tid % lanes < nq ? tid % lanes : nq - 1, step = kSpanThreads / lanes;
+  int lo = kv_len, neg_hi = 0;
+  for (int u = tid / lanes; u < (units + step - 1) / step * step; u += 4 * step) {  // (whole waves: shuffles below)
+    uint32_t x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int at = u + i * step < units ? u + i * step : units - 1;
+      x[i] = rows[(int64_t)q * units + at];
     }
-    int32_t* out = spans + 2 * ((int64_t)b * gridDim.x + blockIdx.x);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int at = u + i * step;
+      uint32_t some = x[i], all = x[i];
+      for (int o = 1; o < lanes; o *= 2) {
+        some |= (uint32_t)__shfl_xor((int)some, o);
+        all &= (uint32_t)__shfl_xor((int)all, o);
+      }
+      if (at >= units) continue;
+      if (some != 0) {
+        const int f = at * kUnit + __ffs((int)some) - 1, e = at * kUnit + 32 - __clz((int)some);
+        lo = f < lo ? f : lo;
+        neg_hi = -e < neg_hi ? -e : neg_hi;
+      }
+      if (all == 0xffffffffu && at < kSpanBits && tid % lanes == 0) atomicOr(&s_full[at / 32], 1u << (at % 32));
+    }
+  }
+  __syncthreads();
+  // first full unit, then the first one behind it that is not
+  auto block_min = [&](int v, int* tmp) {
+    for (int o = 32; o > 0; o >>= 1) {
+      const int w = __shfl_xor(v, o);
+      v = w < v ? w : v;
+    }
+    if ((tid & 63) == 0) tmp[tid >> 6] = v;
+  };
+  auto joined = [&](const int* tmp) {
+    int v = tmp[0];
+    for (int i = 1; i < kSpanThreads / 64; ++i) v = tmp[i] < v ? tmp[i] : v;
+    return v;
+  };
+  const int none = full_words * 32;
+  int full = none;
+  for (int i = tid; i < full_words; i += kSpanThreads)
+    if (s_full[i] != 0) { full = i * 32 + __ffs((int)s_full[i]) - 1; break; }
+  block_min(lo, s_tmp[0]);
+  block_min(neg_hi, s_tmp[1]);
+  block_min(full, s_tmp[2]);
+  __syncthreads();
+  lo = joined(s_tmp[0]);
+  neg_hi = joined(s_tmp[1]);
+  full = joined(s_tmp[2]);
+  int stop = none;
+  for (int i = full / 32 + tid; i < full_words; i += kSpanThreads) {
+    const uint32_t gaps = ~s_full[i] & (i == full / 32 ? ~0u << (full % 32) : ~0u);
+    if (gaps != 0) { stop = i * 32 + __ffs((int)gaps) - 1; break; }
+  }
+  __syncthreads();                                  // (s_tmp is read above)
+  block_min(stop, s_tmp[0]);
+  __syncthreads();
+  if (tid == 0) {
+    stop = joined(s_tmp[0]);
+    int32_t* out = spans + kSpanInts * ((int64_t)b * gridDim.x + blockIdx.x);
     out[0] = lo;
-    out[1] = hi < kv_len ? hi : kv_len;
+    out[1] = -neg_hi < kv_len ? -neg_hi : kv_len;
+    out[2] = full < none ? full * kUnit : 0;
+    out[3] = full < none ? stop * kUnit : 0;
   }
 }
 
@@ -661,18 +932,29 @@ __global__ __launch_bounds__(kSpanThreads) void attn_spans_kernel(const uint64_t
 // ---------------------------------------------------------------------------------------------
 constexpr int kComputeUnits = 256;
 
-// The launch of a shape: row blocks of a tile and how the keys are cut.
-struct Shape { int row_blocks, tiles, piece, max_pieces; };
+#ifndef K1
+#define K1 8
+#endif
+#ifndef K2
+#define K2 4
+#endif
+#ifndef WPS
+#define WPS 1
+#endif
+// The launch of a shape: the workgroup's layout (see attn_quant_kernel) and how the keys are cut.
+enum Layout { kNarrow, kMiddle, kWide };  // 16, 32, 128 rows
+struct Shape { int layout, tile_rows, tiles, piece, max_pieces; };
 Shape shape_of(int batch, int n_heads, int n_kv_heads, int n_q, int kv_len) {
   Shape s;
-  const int64_t rows = (int64_t)n_q * (n_heads / n_kv_heads);
-  s.row_blocks = rows <= 16 ? 1 : 2;
-  s.tiles = (int)rd::ceil_div(rows, 16 * s.row_blocks);
-  const int waves = s.row_blocks == 1 ? 8 : 4;
-  // enough pieces that every compute unit has two workgroups, none shorter than four units per wave
-  const int64_t groups = (int64_t)batch * n_kv_heads * s.tiles;
+  const int64_t rows = (int64_t)n_q * (n_heads / n_kv_heads), slabs = (int64_t)batch * n_kv_heads;
+  s.layout = rows <= 16 ? kNarrow : (slabs * rd::ceil_div(rows, 128) < 2 * kComputeUnits ? kMiddle : kWide);
+  s.tile_rows = s.layout == kNarrow ? 16 : (s.layout == kMiddle ? 32 : 128);
+  s.tiles = (int)rd::ceil_div(rows, s.tile_rows);
+  const int k_waves = s.layout == kNarrow ? K1 : s.layout == kMiddle ? K2 : 4, waves = s.layout == kWide ? 4 : k_waves;
+  const int64_t groups = slabs * s.tiles;
   const int step = waves * kUnit;
-  int64_t pieces = groups >= 2 * kComputeUnits ? 1 : 2 * kComputeUnits / groups;
+  const int64_t want = WPS * 4 * kComputeUnits;
+  int64_t pieces = groups * waves >= want ? 1 : want / (groups * waves);
   const int64_t most = rd::ceil_div(kv_len, 4 * step);
   if (pieces > most) pieces = most;
   s.piece = (int)(rd::ceil_div(rd::ceil_div((int64_t)kv_len + kUnit - 1, pieces), step) * step);
@@ -688,16 +970,17 @@ template <typename T, int BITS, int D>
 void launch(const QuantArgs& a, const Shape& s, hipStream_t stream) {
   const dim3 grid((unsigned)(a.Hkv * (int64_t)s.tiles), (unsigned)(a.B * (int64_t)s.max_pieces));
   rd::ScopedTiming rd_t("attn_quant_kernel", stream);
-  switch (s.row_blocks) {
-    case 1: hipLaunchKernelGGL((attn_quant_kernel<T, BITS, D, 1, 8>), grid, dim3(512), 0, stream, a); break;
-    default: hipLaunchKernelGGL((attn_quant_kernel<T, BITS, D, 2, 4>), grid, dim3(256), 0, stream, a); break;
+  switch (s.layout) {
+    case kNarrow: hipLaunchKernelGGL((attn_quant_kernel<T, BITS, D, 1, 1, K1>), grid, dim3(64 * K1), 0, stream, a); break;
+    case kMiddle: hipLaunchKernelGGL((attn_quant_kernel<T, BITS, D, 2, 1, K2>), grid, dim3(64 * K2), 0, stream, a); break;
+    default: hipLaunchKernelGGL((attn_quant_kernel<T, BITS, D, 2, 4, 1>), grid, dim3(256), 0, stream, a); break;
   }
 }
 
 }  // namespace
 
 extern "C" size_t rd_attn_spans_ints(int batch, int n_q) {
-  return batch > 0 && n_q > 0 ? 2 * (size_t)batch * rd::ceil_div(n_q, kSpanQueries) : 0;
+  return batch > 0 && n_q > 0 ? kSpanInts * (size_t)batch * rd::ceil_div(n_q, kSpanQueries) : 0;
 }
 
 extern "C" int rd_attn_spans(const uint64_t* bits, int batch, int n_q, int kv_len, int32_t* spans, void* stream) {
@@ -772,7 +1055,6 @@ extern "C" int rd_verify_attention_quant(const void* q, const int64_t* q_strides
     a.max_pieces = sh.max_pieces; a.piece = sh.piece;
     a.scale = scale * 1.4426950408889634f;
     a.inv_scale = 1.f / a.scale;
-    const int group_rows = 16 * sh.row_blocks;
     if (sh.max_pieces > 1) {
       const size_t need = rd_verify_attention_quant_workspace_bytes(dtype, batch, n_heads, n_kv_heads, n_q, kv_len, head_dim);
       RD_REQUIRE(workspace && workspace_bytes >= need, RD_EWORKSPACE, "%s: workspace %zu < %zu bytes", who, workspace_bytes, need);
@@ -787,9 +1069,10 @@ extern "C" int rd_verify_attention_quant(const void* q, const int64_t* q_strides
       else { if (head_dim == 64) launch<T, 8, 64>(a, sh, s); else launch<T, 8, 128>(a, sh, s); }
       if (sh.max_pieces > 1) {
         rd::ScopedTiming rd_t("attn_quant_merge_kernel", s);
-        const int64_t n = (int64_t)n_q * a.group * (head_dim / 4);
-        hipLaunchKernelGGL(attn_quant_merge_kernel<T>, dim3((unsigned)rd::ceil_div(n, kMergeThreads), n_kv_heads, batch),
-                           dim3(kMergeThreads), 0, s, a, group_rows);
+        const int parts = sh.max_pieces >= 16 ? kMergeMaxParts : (sh.max_pieces >= 8 ? 4 : 1);
+        const int64_t per_wg = kMergeThreads / (head_dim / 4 * parts);
+        hipLaunchKernelGGL(attn_quant_merge_kernel<T>, dim3((unsigned)rd::ceil_div((int64_t)n_q * a.group, per_wg), n_kv_heads, batch),
+                           dim3(kMergeThreads), 0, s, a, sh.tile_rows, parts);
       }
     };
     if (dtype == RD_BF16) go(__hip_bfloat16{}); else go(__half{});

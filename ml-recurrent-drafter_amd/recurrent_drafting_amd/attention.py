@@ -164,21 +164,22 @@ def _spans(prepared: PreparedMask) -> torch.Tensor:
     A table written while a graph is captured holds nothing before the replay, so it stays with its call."""
     stream = _hip.stream()
     spans = prepared.spans.get(stream)
-    capturing = torch.cuda.is_current_stream_capturing()
-    if spans is None or capturing:
+    if spans is None:
         lib = _hip.lib()
         spans = torch.empty(lib.rd_attn_spans_ints(prepared.batch, prepared.n_q), dtype=torch.int32,
                             device=prepared.bits.device)
         _hip.check(lib.rd_attn_spans(_hip.ptr(prepared.bits), prepared.batch, prepared.n_q, prepared.kv_len,
                                      _hip.ptr(spans), stream))
-        if not capturing:
+        if not torch.cuda.is_current_stream_capturing():
             prepared.spans[stream] = spans
     return spans
 
 
 def _quantized_attention(q, k, v, prepared: PreparedMask, scale, force_generic, rows) -> torch.Tensor:
     """masked_attention over the rows of a cache in 4 or 8 bits (rd_verify_attention_quant)."""
-    assert isinstance(k, kv_cache.QuantizedRows) and isinstance(v, kv_cache.QuantizedRows), "keys and values of one cache"
+    assert isinstance(k, kv_cache.QuantizedRows) and isinstance(v, kv_cache.QuantizedRows) and \
+        k._owner is v._owner, "keys and values of one cache"
+    owner = k._owner
     Bk, Hkv, kv_len, D = k.shape
     if rows is None:
         B, H, n_q, Dq = q.shape
@@ -186,40 +187,39 @@ def _quantized_attention(q, k, v, prepared: PreparedMask, scale, force_generic, 
         T, H, Dq = q.shape
         B, n_q = rows.batch, rows.n
         assert T == rows.rows
-    assert (Bk, D) == (B, Dq) and v.shape == k.shape and (v.bits, v.dtype, v.max_length) == (k.bits, k.dtype, k.max_length)
-    assert q.dtype == k.dtype, "queries in the type the cache was written from"
-    assert list(v.strides()) == list(k.strides())
+    assert (Bk, D) == (B, Dq) and (v._prev, v._length) == (k._prev, k._length)
+    assert q.dtype == owner.dtype, "queries in the type the cache was written from"
     assert (prepared.batch, prepared.n_q, prepared.kv_len) == (B, n_q, kv_len), "mask/plan mismatch"
-    _hip.on_current_device(q, k.records, v.records, prepared.bits)
+    _hip.on_current_device(q, owner._cache, prepared.bits)
     if q.stride(-1) != 1:
         q = q.contiguous()
+    width = H * D
     if rows is None:
-        out = torch.empty((B, n_q, H, D), dtype=q.dtype, device=q.device)
-        q_strides = _strides3(q)
-        o_strides = _strides3(out.permute(0, 2, 1, 3))  # (B, H, n_q, D) strides
+        out = torch.empty((B, n_q, width), dtype=q.dtype, device=q.device)
+        q_strides = _hip.I64x3(*q.stride()[:3])
+        o_strides = _hip.I64x3(n_q * width, D, width)
     else:
-        out = torch.empty((rows.rows, H, D), dtype=q.dtype, device=q.device)
-        q_strides = (C.c_int64 * 3)(0, q.stride(1), q.stride(0))
-        o_strides = (C.c_int64 * 3)(0, out.stride(1), out.stride(0))
+        out = torch.empty((rows.rows, width), dtype=q.dtype, device=q.device)
+        q_strides = _hip.I64x3(0, q.stride(1), q.stride(0))
+        o_strides = _hip.I64x3(0, D, width)
     lib = _hip.lib()
-    dtype = _hip.dtype_code(q.dtype)
     spans = _spans(prepared)
     # partial results of keys cut into pieces: memory of this call alone, so that calls on several
     # streams, or captured in several graphs, may share the mask
-    ws_bytes = lib.rd_verify_attention_quant_workspace_bytes(dtype, B, H, Hkv, n_q, kv_len, D)
+    ws_bytes = lib.rd_verify_attention_quant_workspace_bytes(owner.dtype_code, B, H, Hkv, n_q, kv_len, D)
     workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
     if shape_log is not None:
         shape_log.append((B, n_q, kv_len, B * n_q if rows is None else rows.total))
     _hip.check(
         lib.rd_verify_attention_quant(
-            _hip.ptr(q), q_strides, _hip.ptr(k.records), _hip.ptr(v.records), k.strides(), k.bits, k.max_length,
-            _hip.ptr(out), o_strides, dtype, B, H, Hkv, n_q, kv_len, D,
-            float(scale if scale is not None else 1.0 / math.sqrt(D)), _hip.ptr(prepared.bits),
-            _hip.ptr(prepared.plan), _hip.ptr(spans), _hip.ptr(workspace), ws_bytes,
-            int(force_generic), _hip.ptr(rows.row_start) if rows is not None else None, _hip.stream(),
+            q.data_ptr(), q_strides, k.data_ptr(), v.data_ptr(), owner.byte_strides, owner.bits,
+            owner._cache.shape[4] - k._prev, out.data_ptr(), o_strides, owner.dtype_code, B, H, Hkv, n_q, kv_len, D,
+            1.0 / math.sqrt(D) if scale is None else float(scale), prepared.bits.data_ptr(), prepared.plan.data_ptr(),
+            spans.data_ptr(), workspace.data_ptr() if ws_bytes else None, ws_bytes, int(force_generic),
+            _hip.ptr(rows.row_start) if rows is not None else None, _hip.stream(),
         )
     )
-    return out.view(B, n_q, H * D) if rows is None else out.view(rows.rows, H * D)
+    return out
 
 
 def rope_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,

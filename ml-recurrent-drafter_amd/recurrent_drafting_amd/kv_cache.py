@@ -22,7 +22,6 @@ head_dim 128 where bf16 takes 256.  Rows are rounded as they are written (`rope_
 from __future__ import annotations
 
 import ctypes
-from dataclasses import dataclass
 from typing import Optional, Tuple
 
 import torch
@@ -31,38 +30,57 @@ from . import _hip
 from .packed_rows import PackedRows
 
 
-@dataclass
 class QuantizedRows:
-    """Key or value rows of one layer of a cache held in 4 or 8 bits."""
+    """Key or value rows [prev, length) of one layer of a cache held in 4 or 8 bits."""
 
-    records: torch.Tensor  # (batch, n_heads, length, record bytes) uint8, a view of the cache
-    bits: int
-    head_dim: int
-    dtype: torch.dtype  # the type the rows were rounded from and read back in
-    max_length: int  # rows of a slab of the cache behind the view
+    __slots__ = ("_owner", "_layer", "_kv", "_prev", "_length")
+
+    def __init__(self, owner: "Cache", layer: int, kv: int, prev: int, length: int):
+        self._owner, self._layer, self._kv, self._prev, self._length = owner, layer, kv, prev, length
+
+    @property
+    def bits(self) -> int:
+        return self._owner.bits
+
+    @property
+    def head_dim(self) -> int:
+        return self._owner.head_dim
+
+    @property
+    def dtype(self) -> torch.dtype:
+        """The type the rows were rounded from and are read back in."""
+        return self._owner.dtype
 
     @property
     def shape(self) -> Tuple[int, int, int, int]:
-        return (*self.records.shape[:3], self.head_dim)
+        _, _, batch, n_heads, _, _ = self._owner._cache.shape
+        return (batch, n_heads, self._length - self._prev, self._owner.head_dim)
 
-    def strides(self):
-        """Byte strides {batch, head, row} for the C ABI."""
-        r = self.records
-        return (ctypes.c_int64 * 3)(r.stride(0), r.stride(1), r.stride(2))
+    @property
+    def records(self) -> torch.Tensor:
+        """(batch, n_heads, length - prev, record bytes) uint8, a view of the cache."""
+        return self._owner._cache[self._layer, self._kv, :, :, self._prev : self._length, :]
+
+    def data_ptr(self) -> int:
+        """Address of the first record."""
+        cache = self._owner._cache
+        layer, kv, _, _, row, _ = cache.stride()
+        return cache.data_ptr() + self._layer * layer + self._kv * kv + self._prev * row
 
     def read(self) -> torch.Tensor:
-        """The values, (batch, n_heads, length, head_dim) in `dtype`: exact, every value the records can
-        hold is a number of that type."""
-        batch, n_heads, length, _ = self.records.shape
-        out = torch.empty((batch, n_heads, length, self.head_dim), dtype=self.dtype, device=self.records.device)
-        if out.numel() == 0:
+        """The values, (batch, n_heads, length - prev, head_dim) in `dtype`: exact, every value the records
+        can hold is a number of that type."""
+        owner = self._owner
+        batch, n_heads, n_rows, head_dim = self.shape
+        out = torch.empty((batch, n_heads, n_rows, head_dim), dtype=owner.dtype, device=owner._cache.device)
+        if n_rows == 0 or batch == 0:
             return out
-        _hip.on_current_device(self.records)
+        _hip.on_current_device(out)
+        row = n_rows * head_dim
         _hip.check(
             _hip.lib().rd_kv_dequantize(
-                _hip.ptr(self.records), self.strides(), self.bits, _hip.dtype_code(self.dtype), batch, n_heads, 0,
-                length, self.head_dim, length, _hip.ptr(out),
-                (ctypes.c_int64 * 3)(out.stride(0), out.stride(1), out.stride(2)), _hip.stream(),
+                self.data_ptr(), owner.byte_strides, owner.bits, owner.dtype_code, batch, n_heads, 0, n_rows, head_dim,
+                n_rows, out.data_ptr(), _hip.I64x3(n_heads * row, row, head_dim), _hip.stream(),
             )
         )
         return out
@@ -107,10 +125,9 @@ class View:
             _hip.on_current_device(x, slab)
             _hip.check(
                 _hip.lib().rd_kv_quantize(
-                    _hip.ptr(x), (ctypes.c_int64 * 3)(x.stride(0), x.stride(1), x.stride(2)), _hip.dtype_code(x.dtype),
-                    batch_size, n_heads, n_new, head_dim, self.bits, _hip.ptr(slab),
-                    (ctypes.c_int64 * 3)(slab.stride(0), slab.stride(1), slab.stride(2)), self.length, max_length,
-                    _hip.stream(),
+                    x.data_ptr(), _hip.I64x3(*x.stride()[:3]), self._owner.dtype_code,
+                    batch_size, n_heads, n_new, head_dim, self.bits, slab.data_ptr(),
+                    self._owner.byte_strides, self.length, max_length, _hip.stream(),
                 )
             )
         self.length += n_new
@@ -125,10 +142,9 @@ class View:
         """Rows [prev, length) as the attention reads them: a view of the cache in the model's type, or
         the `QuantizedRows` of one in 4 or 8 bits.  With cache rows in place these are cache rows, not
         token columns (a PreparedMask built with the cache's shifts goes with them)."""
-        rows = self._cache[self._layer, self._kv, :, :, prev : self.length, :]
-        if self.bits is None:
-            return rows
-        return QuantizedRows(rows, self.bits, self._owner.head_dim, self._owner.dtype, self._cache.shape[4] - prev)
+        if self.bits is not None:
+            return QuantizedRows(self._owner, self._layer, self._kv, prev, self.length)
+        return self._cache[self._layer, self._kv, :, :, prev : self.length, :]
 
     def slice(self, prev: int) -> torch.Tensor:
         """Rows [prev, length) (of a cache in 4 or 8 bits: their values, read back)."""
@@ -164,12 +180,12 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Te
     if rows is None:
         n_new = q.shape[1]
         lead = (batch, n_new)
-        strides = lambda t: (ctypes.c_int64 * 2)(t.stride(0), t.stride(1))
+        strides = lambda t: _hip.I64x2(t.stride(0), t.stride(1))
     else:
         assert rows.batch == batch
         n_new = rows.n
         lead = (rows.rows,)
-        strides = lambda t: (ctypes.c_int64 * 2)(0, t.stride(0))
+        strides = lambda t: _hip.I64x2(0, t.stride(0))
     n_heads = q.shape[-1] // head_dim
     assert q.shape == (*lead, n_heads * head_dim) and q.stride(-1) == 1
     assert k.shape == (*lead, n_kv_heads * head_dim) and k.stride(-1) == 1
@@ -179,27 +195,29 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Te
     assert position_ids.shape == (batch, n_new) and position_ids.dtype == torch.long and position_ids.stride(1) == 1
     assert key_view.length == value_view.length and key_view.length + n_new <= max_length
     assert value_view._cache is cache and key_view._layer == value_view._layer
-    k_slab = cache[key_view._layer, 0]
-    v_slab = cache[key_view._layer, 1]
     owner = key_view._owner
     shift = owner.shift if owner is not None and owner.rows_in_place else None
     if bits is not None:
         _hip.on_current_device(q, k, v, cos, sin, position_ids, cache)
-        q_out = torch.empty((*lead, n_heads * head_dim), dtype=q.dtype, device=q.device)
+        q_out = torch.empty((*lead, n_heads, head_dim), dtype=q.dtype, device=q.device)
+        width = n_heads * head_dim
+        keys = QuantizedRows(owner, key_view._layer, 0, 0, key_view.length + n_new)
+        values = QuantizedRows(owner, key_view._layer, 1, 0, key_view.length + n_new)
         _hip.check(
             _hip.lib().rd_rope_append_quant(
-                _hip.ptr(q), strides(q), _hip.ptr(k), strides(k), _hip.ptr(v), strides(v),
-                _hip.dtype_code(q.dtype), batch, n_new, n_heads,
-                n_kv_heads, head_dim, _hip.ptr(cos), _hip.ptr(sin), cos.shape[0], _hip.ptr(position_ids),
-                position_ids.stride(0), _hip.ptr(q_out), strides(q_out), _hip.ptr(k_slab), _hip.ptr(v_slab),
-                (ctypes.c_int64 * 3)(k_slab.stride(0), k_slab.stride(1), k_slab.stride(2)), bits, key_view.length,
-                max_length, _hip.ptr(rows.row_start) if rows is not None else None, _hip.ptr(shift), _hip.stream(),
+                q.data_ptr(), strides(q), k.data_ptr(), strides(k), v.data_ptr(), strides(v),
+                owner.dtype_code, batch, n_new, n_heads, n_kv_heads, head_dim, cos.data_ptr(), sin.data_ptr(),
+                cos.shape[0], position_ids.data_ptr(), position_ids.stride(0), q_out.data_ptr(),
+                _hip.I64x2(n_new * width if rows is None else 0, width), keys.data_ptr(), values.data_ptr(),
+                owner.byte_strides, bits, key_view.length, max_length,
+                _hip.ptr(rows.row_start) if rows is not None else None, _hip.ptr(shift), _hip.stream(),
             )
         )
         key_view.length += n_new
         value_view.length += n_new
-        q_heads = q_out.unflatten(-1, (n_heads, head_dim))
-        return q_heads.transpose(1, 2) if rows is None else q_heads, key_view.rows(), value_view.rows()
+        return q_out.transpose(1, 2) if rows is None else q_out, keys, values
+    k_slab = cache[key_view._layer, 0]
+    v_slab = cache[key_view._layer, 1]
     _hip.check(
         _hip.lib().rd_rope_append(
             _hip.ptr(q), strides(q), _hip.ptr(k), strides(k), _hip.ptr(v), strides(v),
@@ -236,7 +254,7 @@ class Cache:
         self.bits, self.dtype, self.head_dim = bits, dtype, head_dim
         row, element = head_dim, dtype
         if bits is not None:
-            _hip.dtype_code(dtype)
+            self.dtype_code = _hip.dtype_code(dtype)
             row, element = _hip.lib().rd_kv_quant_row_bytes(int(bits), head_dim), torch.uint8
             if bits not in (4, 8) or row == 0:
                 raise ValueError(f"a cache in {bits} bits with head_dim {head_dim}: bits must be 4 or 8, head_dim a "
@@ -245,6 +263,9 @@ class Cache:
         # asked of the memory around a row's live rows; zeros as upstream, kv_cache.py:49-53)
         self._storage = torch.zeros([n_layers, 2, batch_size, n_heads, max_length, row], dtype=element, device=device)
         self._cache = self._storage
+        self.byte_strides = None  # of {batch, head, row} in a layer's keys or values, for the C ABI
+        if bits is not None:
+            self.byte_strides = _hip.I64x3(*self._cache.stride()[2:5])
         self.sliced = tuple(
             (View(self._cache, layer, 0, self), View(self._cache, layer, 1, self)) for layer in range(n_layers)
         )

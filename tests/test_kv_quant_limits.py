@@ -97,7 +97,7 @@ def test_attention_refusals(change, code, word):
 
 def test_spans_and_workspace_sizes():
     lib = _lib()
-    assert lib.rd_attn_spans_ints(3, 1) == 6 and lib.rd_attn_spans_ints(2, 17) == 8 and lib.rd_attn_spans_ints(0, 1) == 0
+    assert lib.rd_attn_spans_ints(3, 1) == 12 and lib.rd_attn_spans_ints(2, 17) == 16 and lib.rd_attn_spans_ints(0, 1) == 0
     assert lib.rd_attn_spans(None, 1, 1, 1, None, None) == EINVAL and lib.rd_attn_spans(FAKE, 0, 1, 1, FAKE, None) == EINVAL
     assert lib.rd_attn_spans(FAKE, 65536, 1, 1, FAKE, None) == ELIMIT
     need = lib.rd_verify_attention_quant_workspace_bytes
