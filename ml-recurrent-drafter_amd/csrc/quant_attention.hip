@@ -208,19 +208,21 @@ __global__ __launch_bounds__(R * K * 64, 2) void attn_quant_kernel(QuantArgs a) 
   constexpr int kMaskAt = kOperandBytes > 2 * kRawBytes ? kOperandBytes : 2 * kRawBytes;
   constexpr int kSlotBytes = kMaskAt + 4 * kRows;
   // a slot per wave (records of K, then of V, or operands), later the rows they merge
-  constexpr int kMergeBytes = K > 1 ? kWaves * 16 * kPitch * 4 : 0;
+  constexpr int kMergeBytes = K > 1 ? kWaves * 16 * RB * kPitch * 4 : 0;
   constexpr int kLdsBytes = kWaves * kSlotBytes > kMergeBytes ? kWaves * kSlotBytes : kMergeBytes;
   __shared__ __attribute__((aligned(16))) char s_mem[kLdsBytes];
-  __shared__ float s_ml[kWaves * 16 * 2];
+  __shared__ float s_ml[kWaves * 16 * RB * 2];
   float* const s_o = reinterpret_cast<float*>(s_mem);
 
-  const int hk = blockIdx.x % a.Hkv, tile = blockIdx.x / a.Hkv;
+  // (a causal prompt's last rows have the most keys: first)
+  const int hk = blockIdx.x % a.Hkv, tile = gridDim.x / a.Hkv - 1 - blockIdx.x / a.Hkv;
   const int b = blockIdx.y / a.max_pieces, piece = blockIdx.y % a.max_pieces;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, grp = lane >> 4;
   const int row_wave = wave % R, key_wave = wave / R;
   const int row0 = tile * kRows;
+  const int shift = a.plan[RD_PLAN_HDR + 4 * b + 3];  // (requested together with what the tile needs)
   const Tile t = tile_of(a, b, row0, kRows);
   if (row0 >= t.rows || piece >= t.n_pieces) return;
   const int lo = t.begin + piece * a.piece;
@@ -229,7 +231,6 @@ __global__ __launch_bounds__(R * K * 64, 2) void attn_quant_kernel(QuantArgs a) 
   // K and V rows of the piece through descriptors that begin at key lo (or at the slab's first row, `skip`
   // keys further, where a shift puts lo in front of it) and end behind the last attended key: rows outside
   // read as zeros without touching memory.
-  const int shift = a.plan[RD_PLAN_HDR + 4 * b + 3];
   const int skip = shift > lo ? shift - lo : 0;
   const int64_t end = hi < a.max_len + shift ? hi : a.max_len + shift;
   const bool any = end > (int64_t)lo + skip;
@@ -240,19 +241,6 @@ __global__ __launch_bounds__(R * K * 64, 2) void attn_quant_kernel(QuantArgs a) 
   const int q_first = row0 / a.group;               // first query of the tile
   const __amdgpu_buffer_rsrc_t mr = __builtin_amdgcn_make_buffer_rsrc(
       const_cast<uint64_t*>(a.bits) + ((int64_t)b * a.n_q + q_first) * a.words, 0, 0x7fffffff, 0x00020000);
-
-  // queries: B operand of the first product, lane (row l % 16, dims of chunk l / 16)
-  u32x4 qf[RB][kSteps];
-#pragma unroll
-  for (int rb = 0; rb < RB; ++rb) {
-    const int r = row0 + 16 * (RB * row_wave + rb) + col;
-    const int rc = r < t.rows ? r : t.rows - 1;     // behind the last row: that row again, not written
-    const int qi = rc / a.group;
-    const int h = hk * a.group + (rc - qi * a.group);
-    const T* qp = reinterpret_cast<const T*>(a.q) + t.q_off + (int64_t)h * a.q_sh + (int64_t)qi * a.q_ss + grp * (D / 4);
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) qf[rb][s] = *reinterpret_cast<const u32x4*>(qp + 8 * s);
-  }
 
   int mask_off[kMaskWords];                         // of the rows whose mask words the lane brings
 #pragma unroll
@@ -403,6 +391,20 @@ __global__ __launch_bounds__(R * K * 64, 2) void attn_quant_kernel(QuantArgs a) 
 #pragma unroll
     for (int j = 0; j < kCols; ++j) dst[64 * (2 * kSteps + j)] = v_operand(p, j);
   };
+  if (any) fetch_first();                           // (ahead of the queries, which are needed later)
+
+  // queries: B operand of the first product, lane (row l % 16, dims of chunk l / 16)
+  u32x4 qf[RB][kSteps];
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) {
+    const int r = row0 + 16 * (RB * row_wave + rb) + col;
+    const int rc = r < t.rows ? r : t.rows - 1;     // behind the last row: that row again, not written
+    const int qi = rc / a.group;
+    const int h = hk * a.group + (rc - qi * a.group);
+    const T* qp = reinterpret_cast<const T*>(a.q) + t.q_off + (int64_t)h * a.q_sh + (int64_t)qi * a.q_ss + grp * (D / 4);
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) qf[rb][s] = *reinterpret_cast<const u32x4*>(qp + 8 * s);
+  }
   const bool active = row0 + 16 * RB * row_wave < t.rows;  // (a wave without rows only brings and converts units)
 
   // o: output tiles, l: row sums (the product of P with ones: every element of a lane's l is its row's sum),
@@ -500,7 +502,6 @@ __global__ __launch_bounds__(R * K * 64, 2) void attn_quant_kernel(QuantArgs a) 
       for (int j = 0; j < kCols; ++j) o[rb][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
     if (!any) return;                               // (uniform over the workgroup)
-    fetch_first();
     if constexpr (!kShared) {
       // Every wave by itself.  While unit i is multiplied with V, unit i + kWaves goes to LDS and its K codes
       // come back, and unit i + 2 kWaves is on its way from memory.
@@ -626,7 +627,10 @@ __global__ __launch_bounds__(R * K * 64, 2) void attn_quant_kernel(QuantArgs a) 
 #pragma unroll
       for (int e = 0; e < 4; ++e) odd_row = odd_row || o[rb][j][e] != o[rb][j][e];
   if constexpr (R > 1) odd_row = __syncthreads_or(odd_row);  // (all of them: the rounds have barriers)
-  if (__builtin_expect(__ballot(odd_row) != 0, 0)) sweep(std::true_type{});
+  if (__builtin_expect(__ballot(odd_row) != 0, 0)) {
+    fetch_first();
+    sweep(std::true_type{});
+  }
 
   // four neighbouring dims of row r: the result, or this piece's part of it (m in log2 units)
   auto put = [&](int r, int dq, f32x4 acc, float top, float sum) __attribute__((always_inline)) {
@@ -657,39 +661,41 @@ __global__ __launch_bounds__(R * K * 64, 2) void attn_quant_kernel(QuantArgs a) 
       }
     }
   } else {
-    // merge the K waves behind each other, 16 rows of every row wave at a time
-    constexpr int kThreads = kWaves * 64, kQuads = D / 4;
+    // merge the K waves behind each other; row of the merge: (wave * RB + row block) * 16 + col
+    constexpr int kThreads = kWaves * 64, kQuads = D / 4, kBlocks = R * RB;
+    __syncthreads();                                // (the units are no longer read)
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
-      __syncthreads();                              // (the units, or the rows before, are no longer read)
-      float* dst = s_o + (wave * 16 + col) * kPitch + 4 * kCols * grp;
+      const int at = (wave * RB + rb) * 16 + col;
+      float* dst = s_o + at * kPitch + 4 * kCols * grp;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
 #pragma unroll
         for (int j = 0; j < kCols; j += 4)
           *reinterpret_cast<f32x4*>(dst + kCols * i + j) = f32x4{o[rb][j][i], o[rb][j + 1][i], o[rb][j + 2][i], o[rb][j + 3][i]};
       }
-      if (grp == 0) { s_ml[(wave * 16 + col) * 2] = m[rb]; s_ml[(wave * 16 + col) * 2 + 1] = l[rb][0]; }
-      __syncthreads();
-      for (int e = tid; e < 16 * R * kQuads; e += kThreads) {
-        const int rr = e / kQuads, dq = (e - rr * kQuads) * 4;  // rr: row wave * 16 + row
-        const int rw = rr / 16, r = row0 + 16 * (RB * rw + rb) + rr % 16;
-        if (r >= t.rows) continue;
-        float top = -INFINITY;
+      if (grp == 0) { s_ml[at * 2] = m[rb]; s_ml[at * 2 + 1] = l[rb][0]; }
+    }
+    __syncthreads();
 #pragma unroll
-        for (int w = 0; w < K; ++w) top = fmaxf(top, s_ml[((w * R) * 16 + rr) * 2]);
-        const float m_use = fmaxf(top, -3.4e38f);
-        float sum = 0.f;
-        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    for (int e0 = 0; e0 < 16 * kBlocks * kQuads; e0 += kThreads) {
+      const int rr = (e0 + tid) / kQuads, dq = (e0 + tid) % kQuads * 4;
+      const int r = row0 + rr;
+      if (r >= t.rows) continue;
+      float top = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < K; ++w) {
-          const int at = w * R * 16 + rr;
-          const float f = fast_exp2(s_ml[at * 2] - m_use);  // a wave without keys: exp2(-inf)
-          sum += f * s_ml[at * 2 + 1];
-          acc += f * *reinterpret_cast<const f32x4*>(s_o + at * kPitch + dq);
-        }
-        put(r, dq, acc, top, sum);
+      for (int w = 0; w < K; ++w) top = fmaxf(top, s_ml[(w * 16 * kBlocks + rr) * 2]);
+      const float m_use = fmaxf(top, -3.4e38f);
+      float sum = 0.f;
+      f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < K; ++w) {
+        const int at = w * 16 * kBlocks + rr;
+        const float f = fast_exp2(s_ml[at * 2] - m_use);  // a wave without keys: exp2(-inf)
+        sum += f * s_ml[at * 2 + 1];
+        acc += f * *reinterpret_cast<const f32x4*>(s_o + at * kPitch + dq);
       }
+      put(r, dq, acc, top, sum);
     }
   }
 }
@@ -932,29 +938,29 @@ __global__ __launch_bounds__(kSpanThreads) void attn_spans_kernel(const uint64_t
 // ---------------------------------------------------------------------------------------------
 constexpr int kComputeUnits = 256;
 
-#ifndef K1
-#define K1 8
-#endif
-#ifndef K2
-#define K2 4
-#endif
-#ifndef WPS
-#define WPS 1
-#endif
 // The launch of a shape: the workgroup's layout (see attn_quant_kernel) and how the keys are cut.
-enum Layout { kNarrow, kMiddle, kWide };  // 16, 32, 128 rows
+enum Layout { kNarrow, kMiddle2, kMiddle4, kWide };
+constexpr int kTileRows[] = {16, 32, 32, 128}, kLayoutWaves[] = {8, 2, 4, 4};
 struct Shape { int layout, tile_rows, tiles, piece, max_pieces; };
 Shape shape_of(int batch, int n_heads, int n_kv_heads, int n_q, int kv_len) {
   Shape s;
   const int64_t rows = (int64_t)n_q * (n_heads / n_kv_heads), slabs = (int64_t)batch * n_kv_heads;
-  s.layout = rows <= 16 ? kNarrow : (slabs * rd::ceil_div(rows, 128) < 2 * kComputeUnits ? kMiddle : kWide);
-  s.tile_rows = s.layout == kNarrow ? 16 : (s.layout == kMiddle ? 32 : 128);
+  // kWide converts a unit once for 128 rows but stops its four waves twice per 128 keys: it pays where
+  // two of its workgroups fill every compute unit (batch 2, prompt of 1900, 32 / 8 heads: 125 us against 138 us
+  // of kMiddle4; batch 8, 32 heads, 115 rows, 735 keys, where it does not: 37 against 34 us of kMiddle2).
+  // Two waves per tile where that alone gives every SIMD two waves (34 against 37 us), else four (batch 8,
+  // 32 heads, 48 rows, 1000 keys: 27 against 34 us).
+  if (rows <= 16) s.layout = kNarrow;
+  else if (slabs * rd::ceil_div(rows, 128) >= 2 * kComputeUnits) s.layout = kWide;
+  else s.layout = slabs * rd::ceil_div(rows, 32) >= 4 * kComputeUnits ? kMiddle2 : kMiddle4;
+  s.tile_rows = kTileRows[s.layout];
   s.tiles = (int)rd::ceil_div(rows, s.tile_rows);
-  const int k_waves = s.layout == kNarrow ? K1 : s.layout == kMiddle ? K2 : 4, waves = s.layout == kWide ? 4 : k_waves;
+  // Keys are cut into pieces only as far as every SIMD needs a wave (a cut costs the partial results and
+  // the merge; two waves per SIMD: batch 8, 32 heads, 20 rows, 1000 keys 30.5 against 24.9 us), none
+  // shorter than four units per wave.
+  const int waves = kLayoutWaves[s.layout], step = waves * kUnit;
   const int64_t groups = slabs * s.tiles;
-  const int step = waves * kUnit;
-  const int64_t want = WPS * 4 * kComputeUnits;
-  int64_t pieces = groups * waves >= want ? 1 : want / (groups * waves);
+  int64_t pieces = groups * waves >= 4 * kComputeUnits ? 1 : 4 * kComputeUnits / (groups * waves);
   const int64_t most = rd::ceil_div(kv_len, 4 * step);
   if (pieces > most) pieces = most;
   s.piece = (int)(rd::ceil_div(rd::ceil_div((int64_t)kv_len + kUnit - 1, pieces), step) * step);
@@ -970,10 +976,12 @@ template <typename T, int BITS, int D>
 void launch(const QuantArgs& a, const Shape& s, hipStream_t stream) {
   const dim3 grid((unsigned)(a.Hkv * (int64_t)s.tiles), (unsigned)(a.B * (int64_t)s.max_pieces));
   rd::ScopedTiming rd_t("attn_quant_kernel", stream);
+  const dim3 block(64 * kLayoutWaves[s.layout]);
   switch (s.layout) {
-    case kNarrow: hipLaunchKernelGGL((attn_quant_kernel<T, BITS, D, 1, 1, K1>), grid, dim3(64 * K1), 0, stream, a); break;
-    case kMiddle: hipLaunchKernelGGL((attn_quant_kernel<T, BITS, D, 2, 1, K2>), grid, dim3(64 * K2), 0, stream, a); break;
-    default: hipLaunchKernelGGL((attn_quant_kernel<T, BITS, D, 2, 4, 1>), grid, dim3(256), 0, stream, a); break;
+    case kNarrow: hipLaunchKernelGGL((attn_quant_kernel<T, BITS, D, 1, 1, 8>), grid, block, 0, stream, a); break;
+    case kMiddle2: hipLaunchKernelGGL((attn_quant_kernel<T, BITS, D, 2, 1, 2>), grid, block, 0, stream, a); break;
+    case kMiddle4: hipLaunchKernelGGL((attn_quant_kernel<T, BITS, D, 2, 1, 4>), grid, block, 0, stream, a); break;
+    default: hipLaunchKernelGGL((attn_quant_kernel<T, BITS, D, 2, 4, 1>), grid, block, 0, stream, a); break;
   }
 }
 
