@@ -128,8 +128,8 @@ struct AppendArgs {
   int n_new, n_heads, n_kv_heads, head_dim;
 };
 
-// One workgroup per (token, batch row).  A rotation task covers one block of the first half of a
-// head and its partner in the second half, a copy task one block of v.
+// One task per thread; grid (token, batch row, tasks of a token).  A rotation task covers one block of the
+// first half of a head and its partner in the second half, a copy task one block of v.
 template <typename T, int BITS>
 __global__ __launch_bounds__(kThreads) void rope_append_quant_kernel(AppendArgs a) {
 #pragma clang fp contract(off)
@@ -162,7 +162,8 @@ __global__ __launch_bounds__(kThreads) void rope_append_quant_kernel(AppendArgs 
   char* vc = a.v_cache + b * a.c_sb + cache_row * a.c_st;
   const int n_tasks = in_cache ? q_tasks + k_tasks + v_tasks : q_tasks;
 
-  for (int task = threadIdx.x; task < n_tasks; task += kThreads) {
+  const int task = blockIdx.z * kThreads + threadIdx.x;
+  if (task < n_tasks) {
     if (task >= q_tasks + k_tasks) {
       const int c = task - q_tasks - k_tasks;
       const int h = c / (D / kBlock), blk = c % (D / kBlock);
@@ -171,7 +172,7 @@ __global__ __launch_bounds__(kThreads) void rope_append_quant_kernel(AppendArgs 
 #pragma unroll
       for (int e = 0; e < kBlock; ++e) f[e] = Elem<T>::load(x.v[e]);
       put_block<BITS>(vc + h * a.c_sh, D, blk, encode<BITS, T>(f));
-      continue;
+      return;
     }
     const bool is_q = task < q_tasks;
     const int c = is_q ? task : task - q_tasks;
@@ -322,8 +323,8 @@ extern "C" int rd_rope_append_quant(const void* q, const int64_t* q_strides, con
              "%s: bad sizes (batch %d n_new %d heads %d kv_heads %d)", who, batch, n_new, n_heads, n_kv_heads);
   RD_REQUIRE(batch <= 65535, RD_ELIMIT, "%s: batch %d > 65535", who, batch);
   if (const int rc = check_format(who, dtype, bits, head_dim)) return rc;
-  RD_REQUIRE(((int64_t)n_heads + 2 * (int64_t)n_kv_heads) * (head_dim / kBlock) <= 2147483647LL - kThreads, RD_ELIMIT,
-             "%s: too many heads (%d + 2 * %d)", who, n_heads, n_kv_heads);
+  const int64_t tasks = ((int64_t)n_heads + 3 * (int64_t)n_kv_heads) * (head_dim / kBlock / 2);
+  RD_REQUIRE(tasks <= 65535LL * kThreads, RD_ELIMIT, "%s: too many heads (%d + 2 * %d)", who, n_heads, n_kv_heads);
   RD_REQUIRE(q && k && v && cos && sin && position_ids && q_out && k_cache && v_cache && q_strides && k_strides &&
                  v_strides && q_out_strides && cache_strides, RD_EINVAL, "%s: null pointer", who);
   RD_REQUIRE(table_rows > 0, RD_EINVAL, "%s: empty cos/sin table", who);
@@ -353,7 +354,8 @@ extern "C" int rd_rope_append_quant(const void* q, const int64_t* q_strides, con
     rd::ScopedTiming rd_t("rope_append_quant_kernel", s);
     dispatch(dtype, bits, [&](auto zero, auto bits_c) {
       using T = decltype(zero);
-      hipLaunchKernelGGL((rope_append_quant_kernel<T, decltype(bits_c)::value>), dim3(n_new, batch), dim3(kThreads), 0, s, a);
+      hipLaunchKernelGGL((rope_append_quant_kernel<T, decltype(bits_c)::value>), dim3(n_new, batch, (unsigned)rd::ceil_div(tasks, kThreads)),
+                         dim3(kThreads), 0, s, a);
     });
   }
   return rd::check_launch(who);
