@@ -172,9 +172,10 @@ __device__ inline Tile tile_of(const QuantArgs& a, int b, int row0, int rows_per
   return t;
 }
 
-// max(a, b) as one instruction (fmaxf first quiets each operand that came out of the matrix pipeline); a NaN
-// may lose, which is fine for a running maximum: its row ends as NaN whatever the maximum
-__device__ inline float larger(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, INFINITY); }
+// max(a, b) as one instruction, with `inf` a register the compiler knows nothing about (fmaxf first quiets
+// each operand that came out of the matrix pipeline, and so does a median with a known infinity); a NaN may
+// lose, which is fine for a running maximum: its row ends as NaN whatever the maximum
+__device__ inline float larger(float a, float b, float inf) { return __builtin_amdgcn_fmed3f(a, b, inf); }
 
 // the lanes l, l ^ 16, l ^ 32, l ^ 48 share a query row
 __device__ inline float row_max(float v) {
@@ -187,6 +188,7 @@ __device__ inline float row_max(float v) {
 // ---------------------------------------------------------------------------------------------
 template <typename T, int BITS, int D, int RB, int R, int K>
 __global__ __launch_bounds__(R * K * 64, 2) void attn_quant_kernel(QuantArgs a) {
+  static_assert(R == 1 || K == 1, "waves side by side or behind each other");
   using O = Ops<T>;
   constexpr int kRec = record_bytes(BITS, D), kCodes = code_bytes(BITS, D);
   constexpr int kSteps = D / 32;                    // blocks of 8 dims in a K chunk
@@ -220,7 +222,7 @@ __global__ __launch_bounds__(R * K * 64, 2) void attn_quant_kernel(QuantArgs a) 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, grp = lane >> 4;
-  const int row_wave = wave % R, key_wave = wave / R;
+  const int row_wave = R > 1 ? wave : 0;
   const int row0 = tile * kRows;
   const int shift = a.plan[RD_PLAN_HDR + 4 * b + 3];  // (requested together with what the tile needs)
   const Tile t = tile_of(a, b, row0, kRows);
@@ -411,6 +413,8 @@ __global__ __launch_bounds__(R * K * 64, 2) void attn_quant_kernel(QuantArgs a) 
   // m: running maximum in log2 units, over: the score above which it is raised
   f32x4 o[RB][kCols], l[RB];
   float m[RB], over[RB];
+  float inf = INFINITY;
+  asm volatile("" : "+v"(inf));
   const u32x4 ones = {O::kOne * 0x10001u, O::kOne * 0x10001u, O::kOne * 0x10001u, O::kOne * 0x10001u};
 
   // mask bits of the wave's rows for the unit whose records lie at `here`
@@ -475,7 +479,7 @@ __global__ __launch_bounds__(R * K * 64, 2) void attn_quant_kernel(QuantArgs a) 
       float x[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) x[j] = sc[rb][j / 4][j % 4];
-      const float top = fmaxf(fmaxf(larger(x[0], x[1]), larger(x[2], x[3])), fmaxf(larger(x[4], x[5]), larger(x[6], x[7])));
+      const float top = fmaxf(fmaxf(larger(x[0], x[1], inf), larger(x[2], x[3], inf)), fmaxf(larger(x[4], x[5], inf), larger(x[6], x[7], inf)));
       if (__ballot(top > over[rb]) != 0) {
         const float up = fmaxf(m[rb], row_max(top) * a.scale);
         const float keep = up == -INFINITY ? 1.f : fast_exp2(m[rb] - up);
@@ -493,6 +497,12 @@ __global__ __launch_bounds__(R * K * 64, 2) void attn_quant_kernel(QuantArgs a) 
     }
   };
 
+  // The queries are waited for here, before the next unit's loads go out: left to its first use, the wait sits
+  // in the loop, where it waits for those loads too, unit after unit.
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) asm volatile("" : "+v"(qf[rb][s]));
   auto sweep = [&](auto check_c) __attribute__((always_inline)) {
     constexpr bool kCheck = decltype(check_c)::value;
 #pragma unroll
@@ -548,22 +558,21 @@ __global__ __launch_bounds__(R * K * 64, 2) void attn_quant_kernel(QuantArgs a) 
         }
       }
     } else {
-      // Rounds: every wave brings and converts one unit (slot = wave), then the R waves side by side go over
-      // the R units of their key wave.
+      // Rounds: every wave brings and converts one unit (slot = wave), then all of them go over the R units.
       for (int round = u0; round < n_units; round += kWaves) {
         __syncthreads();
         stage(round + wave);
         if (round + kWaves < n_units) fetch(round + kWaves + wave);
         if constexpr (!kCheck) convert_slot();
         __syncthreads();
-        const int last = n_units - round < key_wave * R + R ? n_units - round : key_wave * R + R;
+        const int last = n_units - round < R ? n_units - round : R;
         u32x4 kf[2 * kSteps];                       // K operands, requested one unit ahead
         if constexpr (!kCheck) {
 #pragma unroll
-          for (int f = 0; f < 2 * kSteps; ++f) kf[f] = reinterpret_cast<const u32x4*>(s_mem + key_wave * R * kSlotBytes)[64 * f + lane];
+          for (int f = 0; f < 2 * kSteps; ++f) kf[f] = reinterpret_cast<const u32x4*>(s_mem)[64 * f + lane];
         }
         if (!active) continue;
-        for (int slot = key_wave * R; slot < last; ++slot) {
+        for (int slot = 0; slot < last; ++slot) {
           const bool full = is_full(round + slot);
           const char* const here = s_mem + slot * kSlotBytes;
           uint32_t on[RB];
@@ -592,7 +601,7 @@ __global__ __launch_bounds__(R * K * 64, 2) void attn_quant_kernel(QuantArgs a) 
           if constexpr (!kCheck) {
             const u32x4* const ready = reinterpret_cast<const u32x4*>(here) + lane;
 #pragma unroll
-            for (int j = 0; j < kCols; ++j) vf[j] = ready[64 * (2 * kSteps + j)];
+            for (int j = 0; j < kCols / 2; ++j) vf[j] = ready[64 * (2 * kSteps + j)];
             const u32x4* const next = reinterpret_cast<const u32x4*>(s_mem + (slot + 1 < last ? slot + 1 : slot) * kSlotBytes) + lane;
 #pragma unroll
             for (int f = 0; f < 2 * kSteps; ++f) kf[f] = next[64 * f];
@@ -602,6 +611,11 @@ __global__ __launch_bounds__(R * K * 64, 2) void attn_quant_kernel(QuantArgs a) 
           }
           u32x4 pf[RB];
           weights(sc, full, on, pf);
+          if constexpr (!kCheck) {
+            const u32x4* const ready = reinterpret_cast<const u32x4*>(here) + lane;
+#pragma unroll
+            for (int j = kCols / 2; j < kCols; ++j) vf[j] = ready[64 * (2 * kSteps + j)];
+          }
 #pragma unroll
           for (int rb = 0; rb < RB; ++rb) l[rb] = O::mfma(ones, pf[rb], l[rb]);
           VPairs pairs;
@@ -955,14 +969,19 @@ Shape shape_of(int batch, int n_heads, int n_kv_heads, int n_q, int kv_len) {
   else s.layout = slabs * rd::ceil_div(rows, 32) >= 4 * kComputeUnits ? kMiddle2 : kMiddle4;
   s.tile_rows = kTileRows[s.layout];
   s.tiles = (int)rd::ceil_div(rows, s.tile_rows);
-  // Keys are cut into pieces only as far as every SIMD needs a wave (a cut costs the partial results and
-  // the merge; two waves per SIMD: batch 8, 32 heads, 20 rows, 1000 keys 30.5 against 24.9 us), none
-  // shorter than four units per wave.
+  // Keys are cut into pieces as far as every SIMD needs waves: two with few rows, where the kernel waits for
+  // memory (one sequence of 65 536 keys in 8 bits, 8 kv heads: 35 against 44 us), one otherwise (batch 8, 32
+  // heads, 20 rows, 1000 keys: 25 against 30 us).  A piece has at least two (four) units per wave, and a cut
+  // has to save what the merge of the pieces costs, which is about the time of 640 keys (3.5 us; batch 16, 8
+  // kv heads, 1000 keys in two pieces 13.0, in one 10.6 us; one sequence of 2000 keys in four 12.1, in two
+  // 14.4 us).
+  const bool narrow = s.layout == kNarrow;
   const int waves = kLayoutWaves[s.layout], step = waves * kUnit;
-  const int64_t groups = slabs * s.tiles;
-  int64_t pieces = groups * waves >= 4 * kComputeUnits ? 1 : 4 * kComputeUnits / (groups * waves);
-  const int64_t most = rd::ceil_div(kv_len, 4 * step);
-  if (pieces > most) pieces = most;
+  const int64_t have = slabs * s.tiles * waves, want = (narrow ? 8 : 4) * kComputeUnits;
+  const int64_t most = rd::ceil_div(kv_len, (narrow ? 2 : 4) * step);
+  int64_t pieces = have >= want ? 1 : want / have;
+  pieces = pieces < most ? pieces : most;
+  if ((int64_t)kv_len * (pieces - 1) < 640 * pieces) pieces = 1;
   s.piece = (int)(rd::ceil_div(rd::ceil_div((int64_t)kv_len + kUnit - 1, pieces), step) * step);
   s.max_pieces = (int)rd::ceil_div((int64_t)kv_len + kUnit - 1, s.piece);
   return s;
