@@ -542,12 +542,14 @@ __global__ __launch_bounds__(R * K * 64, 2) void attn_quant_kernel(QuantArgs a) 
             sc[rb][1] = O::mfma(k1, qf[rb][s], sc[rb][1]);
           }
         }
+        __builtin_amdgcn_s_setprio(0);
         if constexpr (kCheck) part_nan(c, on);
         u32x4 pf[RB];
         weights(sc, full, on, pf);
         const VPairs pairs = v_pairs(c);
         if (i + kWaves < n_units) next(i + kWaves);
         __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_setprio(1);             // (as below: 8 x 32 heads, 128 queries, 1000 keys: 36.6 -> 34.1 us)
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) l[rb] = O::mfma(ones, pf[rb], l[rb]);
 #pragma unroll
@@ -585,6 +587,10 @@ __global__ __launch_bounds__(R * K * 64, 2) void attn_quant_kernel(QuantArgs a) 
           f32x4 sc[RB][2];
 #pragma unroll
           for (int rb = 0; rb < RB; ++rb) sc[rb][0] = sc[rb][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+          // The wave in the matrix products goes before the one in the softmax on the same SIMD, whose
+          // exponentials fill the gaps; with equal priorities the two tend to be in the same phase
+          // (16 x 32 heads, 128 queries, 8192 keys: 371 -> 347 us).
+          __builtin_amdgcn_s_setprio(1);
 #pragma unroll
           for (int s = 0; s < kSteps; ++s) {
             if constexpr (kCheck) {
@@ -610,7 +616,9 @@ __global__ __launch_bounds__(R * K * 64, 2) void attn_quant_kernel(QuantArgs a) 
             part_nan(c, on);
           }
           u32x4 pf[RB];
+          __builtin_amdgcn_s_setprio(0);
           weights(sc, full, on, pf);
+          __builtin_amdgcn_s_setprio(1);
           if constexpr (!kCheck) {
             const u32x4* const ready = reinterpret_cast<const u32x4*>(here) + lane;
 #pragma unroll
