@@ -195,11 +195,11 @@ def _quantized_attention(q, k, v, prepared: PreparedMask, scale, force_generic, 
         q = q.contiguous()
     width = H * D
     if rows is None:
-        out = torch.empty((B, n_q, width), dtype=q.dtype, device=q.device)
+        out = q.new_empty((B, n_q, width))
         q_strides = _hip.I64x3(*q.stride()[:3])
         o_strides = _hip.I64x3(n_q * width, D, width)
     else:
-        out = torch.empty((rows.rows, width), dtype=q.dtype, device=q.device)
+        out = q.new_empty((rows.rows, width))
         q_strides = _hip.I64x3(0, q.stride(1), q.stride(0))
         o_strides = _hip.I64x3(0, D, width)
     lib = _hip.lib()
@@ -207,7 +207,7 @@ def _quantized_attention(q, k, v, prepared: PreparedMask, scale, force_generic, 
     # partial results of keys cut into pieces: memory of this call alone, so that calls on several
     # streams, or captured in several graphs, may share the mask
     ws_bytes = lib.rd_verify_attention_quant_workspace_bytes(owner.dtype_code, B, H, Hkv, n_q, kv_len, D)
-    workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
+    workspace = q.new_empty(ws_bytes, dtype=torch.uint8) if ws_bytes else None
     if shape_log is not None:
         shape_log.append((B, n_q, kv_len, B * n_q if rows is None else rows.total))
     _hip.check(

@@ -63,19 +63,20 @@ class QuantizedRows:
 
     def data_ptr(self) -> int:
         """Address of the first record."""
-        cache = self._owner._cache
-        layer, kv, _, _, row, _ = cache.stride()
-        return cache.data_ptr() + self._layer * layer + self._kv * kv + self._prev * row
+        owner = self._owner
+        layer, kv, row = owner.slab_strides
+        return owner._cache.data_ptr() + self._layer * layer + self._kv * kv + self._prev * row
 
     def read(self) -> torch.Tensor:
         """The values, (batch, n_heads, length - prev, head_dim) in `dtype`: exact, every value the records
         can hold is a number of that type."""
         owner = self._owner
+        cache = owner._cache
         batch, n_heads, n_rows, head_dim = self.shape
-        out = torch.empty((batch, n_heads, n_rows, head_dim), dtype=owner.dtype, device=owner._cache.device)
+        out = cache.new_empty((batch, n_heads, n_rows, head_dim), dtype=owner.dtype)
         if n_rows == 0 or batch == 0:
             return out
-        _hip.on_current_device(out)
+        _hip.on_current_device(cache)
         row = n_rows * head_dim
         _hip.check(
             _hip.lib().rd_kv_dequantize(
@@ -173,8 +174,9 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Te
     projection's output is left as it was), of which the result is a view; rows behind the last token of
     a packed batch are not written."""
     key_view, value_view = past_key_value
+    if key_view.bits is not None:
+        return _rope_append_quantized(q, k, v, cos, sin, position_ids, key_view, value_view, rows)
     cache = key_view._cache
-    bits = key_view.bits
     batch, n_kv_heads, _, head_dim = key_view.shape
     max_length = cache.shape[4]
     if rows is None:
@@ -190,32 +192,13 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Te
     assert q.shape == (*lead, n_heads * head_dim) and q.stride(-1) == 1
     assert k.shape == (*lead, n_kv_heads * head_dim) and k.stride(-1) == 1
     assert v.shape == k.shape and v.stride(-1) == 1
-    assert q.dtype == k.dtype == v.dtype == (cache.dtype if bits is None else key_view._owner.dtype) == cos.dtype == sin.dtype
+    assert q.dtype == k.dtype == v.dtype == cache.dtype == cos.dtype == sin.dtype
     assert cos.shape == sin.shape and cos.shape[1] == head_dim and cos.is_contiguous() and sin.is_contiguous()
     assert position_ids.shape == (batch, n_new) and position_ids.dtype == torch.long and position_ids.stride(1) == 1
     assert key_view.length == value_view.length and key_view.length + n_new <= max_length
     assert value_view._cache is cache and key_view._layer == value_view._layer
     owner = key_view._owner
     shift = owner.shift if owner is not None and owner.rows_in_place else None
-    if bits is not None:
-        _hip.on_current_device(q, k, v, cos, sin, position_ids, cache)
-        q_out = torch.empty((*lead, n_heads, head_dim), dtype=q.dtype, device=q.device)
-        width = n_heads * head_dim
-        keys = QuantizedRows(owner, key_view._layer, 0, 0, key_view.length + n_new)
-        values = QuantizedRows(owner, key_view._layer, 1, 0, key_view.length + n_new)
-        _hip.check(
-            _hip.lib().rd_rope_append_quant(
-                q.data_ptr(), strides(q), k.data_ptr(), strides(k), v.data_ptr(), strides(v),
-                owner.dtype_code, batch, n_new, n_heads, n_kv_heads, head_dim, cos.data_ptr(), sin.data_ptr(),
-                cos.shape[0], position_ids.data_ptr(), position_ids.stride(0), q_out.data_ptr(),
-                _hip.I64x2(n_new * width if rows is None else 0, width), keys.data_ptr(), values.data_ptr(),
-                owner.byte_strides, bits, key_view.length, max_length,
-                _hip.ptr(rows.row_start) if rows is not None else None, _hip.ptr(shift), _hip.stream(),
-            )
-        )
-        key_view.length += n_new
-        value_view.length += n_new
-        return q_out.transpose(1, 2) if rows is None else q_out, keys, values
     k_slab = cache[key_view._layer, 0]
     v_slab = cache[key_view._layer, 1]
     _hip.check(
@@ -235,6 +218,56 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Te
     else:
         q_heads = q.unflatten(1, (n_heads, head_dim))
     return q_heads, k_slab[:, :, : key_view.length, :], v_slab[:, :, : value_view.length, :]
+
+
+def _rope_append_quantized(q, k, v, cos, sin, position_ids, key_view: View, value_view: View,
+                           rows: Optional[PackedRows]):
+    """rope_append into a cache in 4 or 8 bits (rd_rope_append_quant).  For a single token the kernel takes less
+    time than this function, so every tensor is asked once for what is needed of it."""
+    cache, owner, layer, length = key_view._cache, key_view._owner, key_view._layer, key_view.length
+    _, _, batch, n_kv_heads, max_length, _ = cache.shape
+    head_dim = owner.head_dim
+    q_shape, k_shape, q_stride, k_stride, v_stride = q.shape, k.shape, q.stride(), k.stride(), v.stride()
+    width, kv_width = q_shape[-1], n_kv_heads * head_dim
+    n_heads = width // head_dim
+    n_new = q_shape[1] if rows is None else rows.n
+    if rows is None:
+        assert q_shape == (batch, n_new, n_heads * head_dim) and k_shape == (batch, n_new, kv_width)
+        q_strides, k_strides, v_strides = _hip.I64x2(*q_stride[:2]), _hip.I64x2(*k_stride[:2]), _hip.I64x2(*v_stride[:2])
+    else:
+        assert rows.batch == batch
+        assert q_shape == (rows.rows, n_heads * head_dim) and k_shape == (rows.rows, kv_width)
+        q_strides, k_strides, v_strides = _hip.I64x2(0, q_stride[0]), _hip.I64x2(0, k_stride[0]), _hip.I64x2(0, v_stride[0])
+    assert v.shape == k_shape and q_stride[-1] == k_stride[-1] == v_stride[-1] == 1
+    dtype = q.dtype
+    assert dtype == k.dtype == v.dtype == owner.dtype == cos.dtype == sin.dtype
+    table = cos.shape
+    assert table == sin.shape and table[1] == head_dim and cos.is_contiguous() and sin.is_contiguous()
+    positions = position_ids.stride()
+    assert position_ids.shape == (batch, n_new) and position_ids.dtype == torch.long and positions[1] == 1
+    assert length == value_view.length and length + n_new <= max_length
+    assert value_view._cache is cache and layer == value_view._layer
+    _hip.on_current_device(q, k, v, cos, sin, position_ids, cache)
+    # the result: (batch, heads, n, head_dim), a view of (batch, n, heads, head_dim)
+    if rows is None:
+        q_out = q.new_empty_strided((batch, n_heads, n_new, head_dim), (n_new * width, head_dim, width, 1))
+        out_strides = _hip.I64x2(n_new * width, width)
+    else:
+        q_out = q.new_empty((rows.rows, n_heads, head_dim))
+        out_strides = _hip.I64x2(0, width)
+    keys = QuantizedRows(owner, layer, 0, 0, length + n_new)
+    values = QuantizedRows(owner, layer, 1, 0, length + n_new)
+    _hip.check(
+        _hip.lib().rd_rope_append_quant(
+            q.data_ptr(), q_strides, k.data_ptr(), k_strides, v.data_ptr(), v_strides, owner.dtype_code, batch, n_new,
+            n_heads, n_kv_heads, head_dim, cos.data_ptr(), sin.data_ptr(), table[0], position_ids.data_ptr(),
+            positions[0], q_out.data_ptr(), out_strides, keys.data_ptr(), values.data_ptr(), owner.byte_strides,
+            owner.bits, length, max_length, None if rows is None else _hip.ptr(rows.row_start),
+            _hip.ptr(owner.shift) if owner._rows_in_place else None, _hip.stream(),
+        )
+    )
+    key_view.length = value_view.length = length + n_new
+    return q_out, keys, values
 
 
 class Cache:
@@ -265,7 +298,9 @@ class Cache:
         self._cache = self._storage
         self.byte_strides = None  # of {batch, head, row} in a layer's keys or values, for the C ABI
         if bits is not None:
-            self.byte_strides = _hip.I64x3(*self._cache.stride()[2:5])
+            layer, kv, batch, head, row, _ = self._cache.stride()
+            self.byte_strides = _hip.I64x3(batch, head, row)
+            self.slab_strides = (layer, kv, row)  # bytes from layer to layer, from keys to values, from row to row
         self.sliced = tuple(
             (View(self._cache, layer, 0, self), View(self._cache, layer, 1, self)) for layer in range(n_layers)
         )
