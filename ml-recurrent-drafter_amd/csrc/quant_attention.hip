@@ -141,8 +141,7 @@ struct Tile {
   int n_pieces;     // at least 1: piece 0 of a tile that attends to nothing writes its zeros
   int full_lo, full_hi;  // every row attends to every key of [full_lo, full_hi): whole units, maybe none
 };
-__device__ inline Tile tile_of(const QuantArgs& a, int b, int row0, int rows_per_tile) {
-  Tile t;
+__device__ inline void tile_rows(const QuantArgs& a, int b, Tile& t) {
   int n = a.n_q;
   t.q_off = (int64_t)b * a.q_sb;
   t.o_off = (int64_t)b * a.o_sb;
@@ -154,21 +153,49 @@ __device__ inline Tile tile_of(const QuantArgs& a, int b, int row0, int rows_per
     t.o_off = (int64_t)r0 * a.o_ss;
   }
   t.rows = n * a.group;
+}
+// the keys of the rows from row0 on (kLanes: the span blocks are read by the lanes of a wave, not in turn)
+template <bool kLanes = false>
+__device__ inline void tile_keys(const QuantArgs& a, int b, int row0, int rows_per_tile, Tile& t) {
   t.lo = a.kv_len; t.hi = 0;
   t.full_lo = 0; t.full_hi = a.kv_len;
   if (row0 < t.rows) {
     const int end = row0 + rows_per_tile < t.rows ? row0 + rows_per_tile : t.rows;
     const int s0 = row0 / a.group / kSpanQueries, s1 = (end - 1) / a.group / kSpanQueries;
-    for (int s = s0; s <= s1; ++s) {
-      const int32_t* sp = a.spans + kSpanInts * ((int64_t)b * a.span_blocks + s);
-      t.lo = sp[0] < t.lo ? sp[0] : t.lo;
-      t.hi = sp[1] > t.hi ? sp[1] : t.hi;
-      t.full_lo = sp[2] > t.full_lo ? sp[2] : t.full_lo;
-      t.full_hi = sp[3] < t.full_hi ? sp[3] : t.full_hi;
+    const int32_t* sp = a.spans + kSpanInts * ((int64_t)b * a.span_blocks + s0);
+    if constexpr (kLanes) {
+      const int lane = threadIdx.x & 63;
+      if (lane <= s1 - s0) {
+        const int4 x = reinterpret_cast<const int4*>(sp)[lane];
+        t.lo = x.x; t.hi = x.y; t.full_lo = x.z; t.full_hi = x.w;
+      }
+#pragma unroll
+      for (int x = 1; x < 64; x *= 2) {
+        t.lo = min(t.lo, __shfl_xor(t.lo, x));
+        t.hi = max(t.hi, __shfl_xor(t.hi, x));
+        t.full_lo = max(t.full_lo, __shfl_xor(t.full_lo, x));
+        t.full_hi = min(t.full_hi, __shfl_xor(t.full_hi, x));
+      }
+      t.lo = __builtin_amdgcn_readfirstlane(t.lo);
+      t.hi = __builtin_amdgcn_readfirstlane(t.hi);
+      t.full_lo = __builtin_amdgcn_readfirstlane(t.full_lo);
+      t.full_hi = __builtin_amdgcn_readfirstlane(t.full_hi);
+    } else {
+      for (int s = s0; s <= s1; ++s, sp += kSpanInts) {
+        t.lo = sp[0] < t.lo ? sp[0] : t.lo;
+        t.hi = sp[1] > t.hi ? sp[1] : t.hi;
+        t.full_lo = sp[2] > t.full_lo ? sp[2] : t.full_lo;
+        t.full_hi = sp[3] < t.full_hi ? sp[3] : t.full_hi;
+      }
     }
   }
   t.begin = t.lo / kUnit * kUnit;
   t.n_pieces = t.hi > t.lo ? (t.hi - t.begin + a.piece - 1) / a.piece : 1;
+}
+__device__ inline Tile tile_of(const QuantArgs& a, int b, int row0, int rows_per_tile) {
+  Tile t;
+  tile_rows(a, b, t);
+  tile_keys(a, b, row0, rows_per_tile, t);
   return t;
 }
 
@@ -203,15 +230,20 @@ __global__ __launch_bounds__(R * K * 64, 2) void attn_quant_kernel(QuantArgs a) 
   constexpr int kLoads = (kUnitBytes + 1023) / 1024;  // 16 bytes per lane each
   constexpr int kTail = kUnitBytes / 16 - 64 * (kLoads - 1);  // lanes of the last one that read
   constexpr int kRawBytes = kLoads * 1024;
-  // R > 1: what the waves side by side read of a unit are its operands, converted once: 2 kSteps of K, kCols of V
+  // R > 1: two waves bring a unit, one its K and one its V, and what all of them read of it are its operands,
+  // converted once: 2 kSteps of K, kCols of V.  Two buffers of a round's units each.
   constexpr bool kShared = R > 1;
-  constexpr int kOperandBytes = kShared ? (2 * kSteps + kCols) * 1024 : 0;
-  constexpr int kMaskWords = (kRows + 63) / 64;     // mask words a lane brings for a unit: one per row of the tile
-  constexpr int kMaskAt = kOperandBytes > 2 * kRawBytes ? kOperandBytes : 2 * kRawBytes;
+  constexpr int kRoundUnits = kShared ? R / 2 : K;  // units of a round
+  constexpr int kVAt = kShared ? 2 * kSteps * 1024 : kRawBytes;  // where a slot's V begins, records or operands
+  static_assert(kVAt >= kRawBytes && (!kShared || kCols * 1024 >= kRawBytes), "records fit the place of their operands");
+  constexpr int kMaskRows = kShared ? kRows / 2 : kRows;  // rows of the tile whose mask words a wave brings
+  constexpr int kMaskWords = (kMaskRows + 63) / 64;
+  constexpr int kMaskAt = kShared ? kVAt + kCols * 1024 : 2 * kRawBytes;
   constexpr int kSlotBytes = kMaskAt + 4 * kRows;
-  // a slot per wave (records of K, then of V, or operands), later the rows they merge
+  // the slots (records of K, then of V, or operands), later the rows that waves behind each other merge
+  constexpr int kSlots = kShared ? 2 * kRoundUnits : K;
   constexpr int kMergeBytes = K > 1 ? kWaves * 16 * RB * kPitch * 4 : 0;
-  constexpr int kLdsBytes = kWaves * kSlotBytes > kMergeBytes ? kWaves * kSlotBytes : kMergeBytes;
+  constexpr int kLdsBytes = kSlots * kSlotBytes > kMergeBytes ? kSlots * kSlotBytes : kMergeBytes;
   __shared__ __attribute__((aligned(16))) char s_mem[kLdsBytes];
   __shared__ float s_ml[kWaves * 16 * RB * 2];
   float* const s_o = reinterpret_cast<float*>(s_mem);
@@ -223,10 +255,29 @@ __global__ __launch_bounds__(R * K * 64, 2) void attn_quant_kernel(QuantArgs a) 
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, grp = lane >> 4;
   const int row_wave = R > 1 ? wave : 0;
+  // which unit of a round the wave brings, and (R > 1) whether its K (0) or its V (1)
+  const int mine = kShared ? wave % kRoundUnits : wave, part = kShared ? wave / kRoundUnits : 0;
   const int row0 = tile * kRows;
   const int shift = a.plan[RD_PLAN_HDR + 4 * b + 3];  // (requested together with what the tile needs)
-  const Tile t = tile_of(a, b, row0, kRows);
-  if (row0 >= t.rows || piece >= t.n_pieces) return;
+  Tile t;
+  tile_rows(a, b, t);
+  if (row0 >= t.rows) return;
+
+  // queries: B operand of the first product, lane (row l % 16, dims of chunk l / 16)
+  u32x4 qf[RB][kSteps];
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) {
+    const int r = row0 + 16 * (RB * row_wave + rb) + col;
+    const int rc = r < t.rows ? r : t.rows - 1;     // behind the last row: that row again, not written
+    const int qi = rc / a.group;
+    const int h = hk * a.group + (rc - qi * a.group);
+    const T* qp = reinterpret_cast<const T*>(a.q) + t.q_off + (int64_t)h * a.q_sh + (int64_t)qi * a.q_ss + grp * (D / 4);
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) qf[rb][s] = *reinterpret_cast<const u32x4*>(qp + 8 * s);
+  }
+
+  tile_keys<(kRows > 64)>(a, b, row0, kRows, t);
+  if (piece >= t.n_pieces) return;
   const int lo = t.begin + piece * a.piece;
   const int hi = t.hi < lo + a.piece ? t.hi : lo + a.piece;
 
@@ -247,19 +298,16 @@ __global__ __launch_bounds__(R * K * 64, 2) void attn_quant_kernel(QuantArgs a) 
   int mask_off[kMaskWords];                         // of the rows whose mask words the lane brings
 #pragma unroll
   for (int x = 0; x < kMaskWords; ++x) {
-    const int r = row0 + (lane + 64 * x) % kRows;
+    const int r = row0 + kMaskRows * part + (lane + 64 * x) % kMaskRows;
     mask_off[x] = ((r < t.rows ? r : t.rows - 1) / a.group - q_first) * a.words * 8;
   }
 
   const int n_units = (hi - lo + kUnit - 1) / kUnit;
   const int u0 = skip / kUnit;                      // (0, unless a shift points in front of the slab)
-  // A round: every wave brings one unit into LDS (slot = wave); the R waves side by side go over the R units
-  // of their key wave.  The next round's loads are in flight meanwhile.
-  constexpr uint32_t kStride = kWaves * kUnitBytes, kNowhere = 0x80000000u;  // (beyond every range)
+  constexpr uint32_t kStride = kRoundUnits * kUnitBytes, kNowhere = 0x80000000u;  // (beyond every range)
   uint32_t off_at, tail_at;                         // byte offsets of the lane in the coming unit, and in its last load
-  u32x4 rk[kLoads], rv[kLoads];
-  char* const slot_k = s_mem + wave * kSlotBytes;
-  char* const slot_v = slot_k + kRawBytes;
+  u32x4 rk[kLoads], rv[kLoads];                     // (R > 1: rk alone, of K or V)
+  const __amdgpu_buffer_rsrc_t first = kShared && part != 0 ? vr : kr;
   uint32_t mask[kMaskWords];
   // which units every row of the tile attends to in full: no mask is read for those
   auto is_full = [&](int i) __attribute__((always_inline)) {
@@ -277,26 +325,28 @@ __global__ __launch_bounds__(R * K * 64, 2) void attn_quant_kernel(QuantArgs a) 
 #pragma unroll
     for (int j = 0; j < kLoads; ++j) {
       const uint32_t off = j + 1 < kLoads ? off_at + 1024 * j : tail_at;
-      rk[j] = __builtin_amdgcn_raw_buffer_load_b128(kr, off, 0, 0);
+      rk[j] = __builtin_amdgcn_raw_buffer_load_b128(first, off, 0, 0);
     }
+    if constexpr (!kShared) {
 #pragma unroll
-    for (int j = 0; j < kLoads; ++j) {
-      const uint32_t off = j + 1 < kLoads ? off_at + 1024 * j : tail_at;
-      rv[j] = __builtin_amdgcn_raw_buffer_load_b128(vr, off, 0, 0);
+      for (int j = 0; j < kLoads; ++j) {
+        const uint32_t off = j + 1 < kLoads ? off_at + 1024 * j : tail_at;
+        rv[j] = __builtin_amdgcn_raw_buffer_load_b128(vr, off, 0, 0);
+      }
     }
     off_at += kStride; tail_at += kStride;
     asm volatile("" : "+v"(off_at), "+v"(tail_at));
   };
   auto fetch_first = [&]() __attribute__((always_inline)) {
-    const int base = ((u0 + wave) * kUnit - skip) * kRec + 16 * lane;  // (negative for rows in front of the slab)
+    const int base = ((u0 + mine) * kUnit - skip) * kRec + 16 * lane;  // (negative for rows in front of the slab)
 #pragma unroll
     for (int j = 0; j < kLoads; ++j) {
       const int at = base + 1024 * j;
       const uint32_t off = at < 0 || (j + 1 == kLoads && lane >= kTail) ? kNowhere : (uint32_t)at;
-      rk[j] = __builtin_amdgcn_raw_buffer_load_b128(kr, off, 0, 0);
-      rv[j] = __builtin_amdgcn_raw_buffer_load_b128(vr, off, 0, 0);
+      rk[j] = __builtin_amdgcn_raw_buffer_load_b128(first, off, 0, 0);
+      if constexpr (!kShared) rv[j] = __builtin_amdgcn_raw_buffer_load_b128(vr, off, 0, 0);
     }
-    fetch_mask(u0 + wave);
+    fetch_mask(u0 + mine);
     off_at = (uint32_t)base + kStride;
     tail_at = lane < kTail ? (uint32_t)base + 1024 * (kLoads - 1) + kStride : kNowhere;
     asm volatile("" : "+v"(off_at), "+v"(tail_at));
@@ -308,15 +358,19 @@ __global__ __launch_bounds__(R * K * 64, 2) void attn_quant_kernel(QuantArgs a) 
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
   };
-  auto stage = [&](int i) __attribute__((always_inline)) {
+  auto stage = [&](int i, char* slot) __attribute__((always_inline)) {
+    char* const at = slot + (kShared ? part * kVAt : 0) + 16 * lane;
 #pragma unroll
-    for (int j = 0; j < kLoads; ++j) *reinterpret_cast<u32x4*>(slot_k + 1024 * j + 16 * lane) = rk[j];
+    for (int j = 0; j < kLoads; ++j) *reinterpret_cast<u32x4*>(at + 1024 * j) = rk[j];
+    if constexpr (!kShared) {
 #pragma unroll
-    for (int j = 0; j < kLoads; ++j) *reinterpret_cast<u32x4*>(slot_v + 1024 * j + 16 * lane) = rv[j];
+      for (int j = 0; j < kLoads; ++j) *reinterpret_cast<u32x4*>(at + kVAt + 1024 * j) = rv[j];
+    }
     if (i < n_units && !is_full(i)) {
 #pragma unroll
       for (int x = 0; x < kMaskWords; ++x)
-        if (kRows % 64 == 0 || lane + 64 * x < kRows) *reinterpret_cast<uint32_t*>(slot_k + kMaskAt + 4 * (lane + 64 * x)) = mask[x];
+        if (kMaskRows % 64 == 0 || lane + 64 * x < kMaskRows)
+          *reinterpret_cast<uint32_t*>(slot + kMaskAt + 4 * (kMaskRows * part + lane + 64 * x)) = mask[x];
     }
   };
   // the lane's codes and scales of a unit's records, for the operands of the two products
@@ -376,37 +430,29 @@ __global__ __launch_bounds__(R * K * 64, 2) void attn_quant_kernel(QuantArgs a) 
       r[e] = __builtin_amdgcn_perm(p.w[2 * e + 1][j / 2], p.w[2 * e][j / 2], j % 2 == 0 ? 0x05040100u : 0x07060302u);
     return r;
   };
-  // the wave's slot: records -> operands, in the order the lanes read them back
-  auto convert_slot = [&]() __attribute__((always_inline)) {
+  // the wave's part of a slot: records -> operands, in the order the lanes read them back
+  auto convert_part = [&](char* slot) __attribute__((always_inline)) {
     Codes c;
     own_order();
-    k_codes(slot_k, c);
-    v_codes(slot_v, c);
-    own_order();
-    u32x4* const dst = reinterpret_cast<u32x4*>(slot_k) + lane;
+    u32x4* const dst = reinterpret_cast<u32x4*>(slot) + lane;
+    if (part == 0) {
+      k_codes(slot, c);
+      own_order();
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      dst[64 * (2 * s)] = k_operand(c, s, 0);
-      dst[64 * (2 * s + 1)] = k_operand(c, s, 1);
+      for (int s = 0; s < kSteps; ++s) {
+        dst[64 * (2 * s)] = k_operand(c, s, 0);
+        dst[64 * (2 * s + 1)] = k_operand(c, s, 1);
+      }
+    } else {
+      v_codes(slot + kVAt, c);
+      own_order();
+      const VPairs p = v_pairs(c);
+#pragma unroll
+      for (int j = 0; j < kCols; ++j) dst[64 * (2 * kSteps + j)] = v_operand(p, j);
     }
-    const VPairs p = v_pairs(c);
-#pragma unroll
-    for (int j = 0; j < kCols; ++j) dst[64 * (2 * kSteps + j)] = v_operand(p, j);
   };
-  if (any) fetch_first();                           // (ahead of the queries, which are needed later)
+  if (any) fetch_first();
 
-  // queries: B operand of the first product, lane (row l % 16, dims of chunk l / 16)
-  u32x4 qf[RB][kSteps];
-#pragma unroll
-  for (int rb = 0; rb < RB; ++rb) {
-    const int r = row0 + 16 * (RB * row_wave + rb) + col;
-    const int rc = r < t.rows ? r : t.rows - 1;     // behind the last row: that row again, not written
-    const int qi = rc / a.group;
-    const int h = hk * a.group + (rc - qi * a.group);
-    const T* qp = reinterpret_cast<const T*>(a.q) + t.q_off + (int64_t)h * a.q_sh + (int64_t)qi * a.q_ss + grp * (D / 4);
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) qf[rb][s] = *reinterpret_cast<const u32x4*>(qp + 8 * s);
-  }
   const bool active = row0 + 16 * RB * row_wave < t.rows;  // (a wave without rows only brings and converts units)
 
   // o: output tiles, l: row sums (the product of P with ones: every element of a lane's l is its row's sum),
@@ -515,21 +561,22 @@ __global__ __launch_bounds__(R * K * 64, 2) void attn_quant_kernel(QuantArgs a) 
     if constexpr (!kShared) {
       // Every wave by itself.  While unit i is multiplied with V, unit i + kWaves goes to LDS and its K codes
       // come back, and unit i + 2 kWaves is on its way from memory.
+      char* const slot = s_mem + wave * kSlotBytes;
       int i = u0 + wave;
       Codes c;
       auto next = [&](int n) __attribute__((always_inline)) {
         own_order();
-        stage(n);
+        stage(n, slot);
         if (n + kWaves < n_units) fetch(n + kWaves);
         own_order();
-        k_codes(slot_k, c);
+        k_codes(slot, c);
       };
       if (i < n_units) next(i);
       for (; i < n_units; i += kWaves) {
         const bool full = is_full(i);
         uint32_t on[RB];
-        read_mask(slot_k, full, on);
-        v_codes(slot_v, c);
+        read_mask(slot, full, on);
+        v_codes(slot + kVAt, c);
         f32x4 sc[RB][2];
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) sc[rb][0] = sc[rb][1] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -560,29 +607,41 @@ __global__ __launch_bounds__(R * K * 64, 2) void attn_quant_kernel(QuantArgs a) 
         }
       }
     } else {
-      // Rounds: every wave brings and converts one unit (slot = wave), then all of them go over the R units.
-      for (int round = u0; round < n_units; round += kWaves) {
+      // Rounds of kRoundUnits units, which every wave goes over.  Meanwhile it brings its part of the coming
+      // round into the other buffer: those with K before the first unit, those with V, which share their
+      // SIMDs, in the middle of the round.
+      auto bring = [&](int round, int buffer) __attribute__((always_inline)) {
+        char* const slot = s_mem + (buffer * kRoundUnits + mine) * kSlotBytes;
+        __builtin_amdgcn_s_setprio(0);
+        stage(round + mine, slot);
+        if (round + kRoundUnits < n_units) fetch(round + kRoundUnits + mine);
+        if constexpr (!kCheck) convert_part(slot);
+      };
+      __syncthreads();                              // (the first sweep's units are no longer read)
+      bring(u0, 0);
+      int buffer = 0;
+      for (int round = u0; round < n_units; round += kRoundUnits, buffer ^= 1) {
         __syncthreads();
-        stage(round + wave);
-        if (round + kWaves < n_units) fetch(round + kWaves + wave);
-        if constexpr (!kCheck) convert_slot();
-        __syncthreads();
-        const int last = n_units - round < R ? n_units - round : R;
+        const int last = n_units - round < kRoundUnits ? n_units - round : kRoundUnits;
+        const bool more = round + kRoundUnits < n_units;
+        const char* const units = s_mem + buffer * kRoundUnits * kSlotBytes;
+        if (more && (part == 0 || !active)) bring(round + kRoundUnits, buffer ^ 1);
         u32x4 kf[2 * kSteps];                       // K operands, requested one unit ahead
         if constexpr (!kCheck) {
 #pragma unroll
-          for (int f = 0; f < 2 * kSteps; ++f) kf[f] = reinterpret_cast<const u32x4*>(s_mem)[64 * f + lane];
+          for (int f = 0; f < 2 * kSteps; ++f) kf[f] = reinterpret_cast<const u32x4*>(units)[64 * f + lane];
         }
         if (!active) continue;
         for (int slot = 0; slot < last; ++slot) {
+          if (more && part != 0 && slot == kRoundUnits / 2) bring(round + kRoundUnits, buffer ^ 1);
           const bool full = is_full(round + slot);
-          const char* const here = s_mem + slot * kSlotBytes;
+          const char* const here = units + slot * kSlotBytes;
           uint32_t on[RB];
           read_mask(here, full, on);
           Codes c;
           if constexpr (kCheck) {
             k_codes(here, c);
-            v_codes(here + kRawBytes, c);
+            v_codes(here + kVAt, c);
           }
           f32x4 sc[RB][2];
 #pragma unroll
@@ -608,7 +667,7 @@ __global__ __launch_bounds__(R * K * 64, 2) void attn_quant_kernel(QuantArgs a) 
             const u32x4* const ready = reinterpret_cast<const u32x4*>(here) + lane;
 #pragma unroll
             for (int j = 0; j < kCols / 2; ++j) vf[j] = ready[64 * (2 * kSteps + j)];
-            const u32x4* const next = reinterpret_cast<const u32x4*>(s_mem + (slot + 1 < last ? slot + 1 : slot) * kSlotBytes) + lane;
+            const u32x4* const next = reinterpret_cast<const u32x4*>(units + (slot + 1 < last ? slot + 1 : slot) * kSlotBytes) + lane;
 #pragma unroll
             for (int f = 0; f < 2 * kSteps; ++f) kf[f] = next[64 * f];
             __builtin_amdgcn_sched_barrier(0);      // (requested here, so that the softmax covers the way)
@@ -654,35 +713,53 @@ __global__ __launch_bounds__(R * K * 64, 2) void attn_quant_kernel(QuantArgs a) 
     sweep(std::true_type{});
   }
 
-  // four neighbouring dims of row r: the result, or this piece's part of it (m in log2 units)
-  auto put = [&](int r, int dq, f32x4 acc, float top, float sum) __attribute__((always_inline)) {
-    if (t.n_pieces > 1) {
-      const int64_t slot = ((int64_t)b * a.Hkv + hk) * a.max_pieces + piece;
-      const int64_t pr = slot * ((int64_t)a.n_q * a.group) + r;
-      *reinterpret_cast<f32x4*>(a.part_o + pr * D + dq) = acc;
-      if (dq == 0) { a.part_ml[2 * pr] = top; a.part_ml[2 * pr + 1] = sum; }
-    } else {
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;  // (a NaN sum stays one)
-      const int qi = r / a.group, h = hk * a.group + (r - qi * a.group);
-      T* op = reinterpret_cast<T*>(a.out) + t.o_off + (int64_t)h * a.o_sh + (int64_t)qi * a.o_ss + dq;
-      const u32x2 w = {O::pack(acc[0] * inv, acc[1] * inv), O::pack(acc[2] * inv, acc[3] * inv)};
-      *reinterpret_cast<u32x2*>(op) = w;
-    }
-  };
+  // A lane holds the dims [4 kCols grp, 4 kCols (grp + 1)) of its rows.
   if constexpr (K == 1) {
-    // a lane holds the dims [4 kCols grp, 4 kCols (grp + 1)) of its rows
+    // The finished rows (keys are not cut here) go through LDS, from where the lanes write whole rows one behind
+    // the other (the epilogue of 256 rows of 128 dims: 7.9 -> 2 us).
+    typedef u32x4 u32x4_any __attribute__((aligned(8)));
+    constexpr int kOutPitch = 2 * D + 16, kRowLanes = D / 8, kStepRows = 64 / kRowLanes;
+    static_assert(kWaves * 16 * RB * kOutPitch <= kLdsBytes, "LDS of the finished rows");
+    char* const rows = s_mem + wave * 16 * RB * kOutPitch;
+    __syncthreads();                                // (the units are no longer read)
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
-      const int r = row0 + 16 * (RB * row_wave + rb) + col;
+      const float sum = l[rb][0], inv = sum == 0.f ? 0.f : 1.f / sum;  // (a NaN sum stays one)
+      float x[4 * kCols];                           // (the lane's dims in their order)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < kCols; ++j) x[kCols * i + j] = o[rb][j][i] * inv;
+#pragma unroll
+      for (int c = 0; c < 4 * kCols; c += 8)
+        *reinterpret_cast<u32x4*>(rows + (16 * rb + col) * kOutPitch + 2 * (4 * kCols * grp + c)) =
+            u32x4{O::pack(x[c], x[c + 1]), O::pack(x[c + 2], x[c + 3]), O::pack(x[c + 4], x[c + 5]), O::pack(x[c + 6], x[c + 7])};
+    }
+    own_order();
+#pragma unroll
+    for (int r0 = 0; r0 < 16 * RB; r0 += kStepRows) {
+      const int rr = r0 + lane / kRowLanes, r = row0 + 16 * RB * row_wave + rr;
       if (r >= t.rows) continue;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-#pragma unroll
-        for (int j = 0; j < kCols; j += 4)
-          put(r, 4 * kCols * grp + kCols * i + j, f32x4{o[rb][j][i], o[rb][j + 1][i], o[rb][j + 2][i], o[rb][j + 3][i]}, m[rb], l[rb][0]);
-      }
+      const int qi = r / a.group, h = hk * a.group + (r - qi * a.group);
+      T* op = reinterpret_cast<T*>(a.out) + t.o_off + (int64_t)h * a.o_sh + (int64_t)qi * a.o_ss + lane % kRowLanes * 8;
+      *reinterpret_cast<u32x4_any*>(op) = *reinterpret_cast<const u32x4*>(rows + rr * kOutPitch + 16 * (lane % kRowLanes));
     }
   } else {
+    // four neighbouring dims of row r: the result, or this piece's part of it (m in log2 units)
+    auto put = [&](int r, int dq, f32x4 acc, float top, float sum) __attribute__((always_inline)) {
+      if (t.n_pieces > 1) {
+        const int64_t slot = ((int64_t)b * a.Hkv + hk) * a.max_pieces + piece;
+        const int64_t pr = slot * ((int64_t)a.n_q * a.group) + r;
+        *reinterpret_cast<f32x4*>(a.part_o + pr * D + dq) = acc;
+        if (dq == 0) { a.part_ml[2 * pr] = top; a.part_ml[2 * pr + 1] = sum; }
+      } else {
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;  // (a NaN sum stays one)
+        const int qi = r / a.group, h = hk * a.group + (r - qi * a.group);
+        T* op = reinterpret_cast<T*>(a.out) + t.o_off + (int64_t)h * a.o_sh + (int64_t)qi * a.o_ss + dq;
+        const u32x2 w = {O::pack(acc[0] * inv, acc[1] * inv), O::pack(acc[2] * inv, acc[3] * inv)};
+        *reinterpret_cast<u32x2*>(op) = w;
+      }
+    };
     // merge the K waves behind each other; row of the merge: (wave * RB + row block) * 16 + col
     constexpr int kThreads = kWaves * 64, kQuads = D / 4, kBlocks = R * RB;
     __syncthreads();                                // (the units are no longer read)
@@ -962,19 +1039,25 @@ constexpr int kComputeUnits = 256;
 
 // The launch of a shape: the workgroup's layout (see attn_quant_kernel) and how the keys are cut.
 enum Layout { kNarrow, kMiddle2, kMiddle4, kWide };
-constexpr int kTileRows[] = {16, 32, 32, 128}, kLayoutWaves[] = {8, 2, 4, 4};
+constexpr int kTileRows[] = {16, 32, 32, 256}, kLayoutWaves[] = {8, 2, 4, 8};
 struct Shape { int layout, tile_rows, tiles, piece, max_pieces; };
 Shape shape_of(int batch, int n_heads, int n_kv_heads, int n_q, int kv_len) {
   Shape s;
   const int64_t rows = (int64_t)n_q * (n_heads / n_kv_heads), slabs = (int64_t)batch * n_kv_heads;
-  // kWide converts a unit once for 128 rows but stops its four waves twice per 128 keys: it pays where
-  // two of its workgroups fill every compute unit (batch 2, prompt of 1900, 32 / 8 heads: 125 us against 138 us
-  // of kMiddle4; batch 8, 32 heads, 115 rows, 735 keys, where it does not: 37 against 34 us of kMiddle2).
+  // kWide converts a unit once for 256 rows, in one workgroup of eight waves on a compute unit.  It is the faster
+  // one (batch 2, prompt of 1900, 32 / 8 heads: 87 us against 110 us) where its workgroups come out even, that is
+  // where rows fill three quarters of what whole rounds of them hold: batch 8, 32 heads, 1200 keys in 4 bits,
+  // 162 rows (0.75) 51 against 63 us, 128 rows (0.5) 42 against 37 us; batch 12, 128 rows over 1500 keys (0.38) 60
+  // against 50 us.  Prompts wait for the longest of their tiles, which the first round has; they need a quarter of a
+  // round more: batch 2, 32 / 8 heads, 1300 tokens (1.3 rounds) 55 against 62 us, batch 1, 2000 tokens (1 round) 75
+  // against 61 us.
   // Two waves per tile where that alone gives every SIMD two waves (34 against 37 us), else four (batch 8,
   // 32 heads, 48 rows, 1000 keys: 27 against 34 us).
+  const int64_t wide = slabs * rd::ceil_div(rows, 256), blocks = slabs * rd::ceil_div(rows, 32);
+  const bool prompt = n_q > kv_len / 2;
   if (rows <= 16) s.layout = kNarrow;
-  else if (slabs * rd::ceil_div(rows, 128) >= 2 * kComputeUnits) s.layout = kWide;
-  else s.layout = slabs * rd::ceil_div(rows, 32) >= 4 * kComputeUnits ? kMiddle2 : kMiddle4;
+  else if (prompt ? 4 * wide >= 5 * kComputeUnits : 4 * blocks >= 3 * 8 * kComputeUnits * rd::ceil_div(wide, kComputeUnits)) s.layout = kWide;
+  else s.layout = blocks >= 4 * kComputeUnits ? kMiddle2 : kMiddle4;
   s.tile_rows = kTileRows[s.layout];
   s.tiles = (int)rd::ceil_div(rows, s.tile_rows);
   // Keys are cut into pieces as far as every SIMD needs waves: two with few rows, where the kernel waits for
@@ -987,7 +1070,7 @@ Shape shape_of(int batch, int n_heads, int n_kv_heads, int n_q, int kv_len) {
   const int waves = kLayoutWaves[s.layout], step = waves * kUnit;
   const int64_t have = slabs * s.tiles * waves, want = (narrow ? 8 : 4) * kComputeUnits;
   const int64_t most = rd::ceil_div(kv_len, (narrow ? 2 : 4) * step);
-  int64_t pieces = have >= want ? 1 : want / have;
+  int64_t pieces = have >= want ? 1 : want / have;  // (kWide: 1, it has 192 workgroups or more)
   pieces = pieces < most ? pieces : most;
   if ((int64_t)kv_len * (pieces - 1) < 640 * pieces) pieces = 1;
   s.piece = (int)(rd::ceil_div(rd::ceil_div((int64_t)kv_len + kUnit - 1, pieces), step) * step);
@@ -1008,7 +1091,7 @@ void launch(const QuantArgs& a, const Shape& s, hipStream_t stream) {
     case kNarrow: hipLaunchKernelGGL((attn_quant_kernel<T, BITS, D, 1, 1, 8>), grid, block, 0, stream, a); break;
     case kMiddle2: hipLaunchKernelGGL((attn_quant_kernel<T, BITS, D, 2, 1, 2>), grid, block, 0, stream, a); break;
     case kMiddle4: hipLaunchKernelGGL((attn_quant_kernel<T, BITS, D, 2, 1, 4>), grid, block, 0, stream, a); break;
-    default: hipLaunchKernelGGL((attn_quant_kernel<T, BITS, D, 2, 4, 1>), grid, block, 0, stream, a); break;
+    default: hipLaunchKernelGGL((attn_quant_kernel<T, BITS, D, 2, 8, 1>), grid, block, 0, stream, a); break;
   }
 }
 
@@ -1063,7 +1146,7 @@ extern "C" int rd_verify_attention_quant(const void* q, const int64_t* q_strides
   RD_REQUIRE(max_len > 0, RD_EINVAL, "%s: empty cache", who);
   RD_REQUIRE(scale > 0.f && scale <= 3.402823466e38f, RD_EINVAL, "%s: scale %g is not a positive finite number", who, (double)scale);
   auto al = [](const void* p, int n) { return ((uintptr_t)p & (n - 1)) == 0; };
-  RD_REQUIRE(al(k_cache, 16) && al(v_cache, 16), RD_EINVAL, "%s: the cache must be 16-byte aligned", who);
+  RD_REQUIRE(al(k_cache, 16) && al(v_cache, 16) && al(spans, 16), RD_EINVAL, "%s: the cache and the spans must be 16-byte aligned", who);
   RD_REQUIRE(cache_strides[0] % 16 == 0 && cache_strides[1] % 16 == 0 && cache_strides[0] >= 0 && cache_strides[1] >= 0 &&
                  cache_strides[2] == record_bytes(bits, head_dim), RD_EINVAL,
              "%s: cache strides must be multiples of 16 bytes and rows %d bytes apart", who, record_bytes(bits, head_dim));

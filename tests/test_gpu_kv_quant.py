@@ -385,6 +385,106 @@ def test_one_long_row_is_cut_into_pieces():
         mask[0, 1, 12000:] = False
         _check(q, cache, k, v, mask, dtype)
 
+# ---- launches large enough for the layouts with many rows ---------------------------------------------
+
+def _repeated(q, k, v, batch, copies, dtype, bits):
+    """The two sequences and two kv heads of q, k and v over `batch` rows and 2 * copies kv heads, in a cache
+    whose other rows are filled with 0xFF."""
+    rep = lambda x: x[torch.arange(batch) % 2].repeat(1, copies, 1, 1).cuda()
+    cache = _new(batch, k.shape[2] + 3, 2 * copies, k.shape[3], dtype, bits)
+    cache._cache.fill_(0xFF)
+    for view, x in zip(cache.sliced[0], (k, v)):
+        view.append(rep(x))
+    return rep(q), cache
+
+
+LARGE = [  # batch, kv heads, group, n_q, prev, mask
+    (8, 24, 1, 230, 300, "tree"), (13, 16, 2, 121, 133, "tree"), (10, 8, 4, 225, 0, "causal"), (8, 32, 1, 115, 150, "tree"),
+    (16, 20, 1, 250, 20, "causal"), (9, 64, 1, 255, 260, "scattered")]
+
+
+@pytest.mark.parametrize("dtype,bits,dim", [(torch.bfloat16, 4, 128), (torch.float16, 8, 64), (torch.bfloat16, 8, 128), (torch.float16, 4, 64)])
+@pytest.mark.parametrize("batch,kv_heads,group,n,prev,kind", LARGE)
+@pytest.mark.parametrize("poisoned", [False, True])
+def test_large_launches(batch, kv_heads, group, n, prev, kind, dtype, bits, dim, poisoned):
+    """Two sequences and two kv heads against the oracle, and every copy of them over the batch and the heads
+    with the same bits.  Poisoned: NaN blocks that some rows attend to and that nobody attends to."""
+    from recurrent_drafting_amd import attention
+
+    rng = np.random.default_rng(1000 * n + batch)
+    kv = prev + n
+    x = rng.standard_normal((2, 2, 2, kv, dim))
+    pads = [0, kv // 5]
+    if kind == "tree":
+        mask = _tree_mask(rng, 2, n, prev, pads)
+    else:
+        mask = np.broadcast_to(np.tril(np.ones((n, kv), bool), prev), (2, n, kv)).copy()
+        mask[1, :, : pads[1]] = False  # (of a prompt's second sequence the first rows attend to nothing)
+        if kind == "scattered":
+            mask &= rng.random(mask.shape) < 0.2
+    if poisoned:
+        x[1, 0, 0, 40, 9], x[1, 1, 1, kv - 2, dim - 1], x[0, 1, 0, kv // 2, 5] = np.nan, np.inf, np.nan
+        mask[0, :, 40] = False                        # V: nobody
+        mask[1, : n - 3, kv - 2] = False              # V: some of the last rows
+        mask[1, n // 2 :, kv // 2] = False            # K: some of the first rows
+    k, v = (torch.tensor(t).to(dtype) for t in x)
+    q = torch.tensor(2 * rng.standard_normal((2, 2 * group, n, dim))).to(dtype)
+    big_q, cache = _repeated(q, k, v, batch, kv_heads // 2, dtype, bits)
+    prepared = attention.prepare(torch.tensor(mask[np.arange(batch) % 2]).cuda(), fix_empty_rows=False, n_heads=kv_heads * group)
+    out = attention.masked_attention(big_q, cache.sliced[0][0].rows(), cache.sliced[0][1].rows(), prepared)
+    out = out.view(batch, n, kv_heads // 2, 2 * group, dim)
+    same = out[torch.arange(batch) % 2, :, :1].expand_as(out)
+    assert torch.equal(out.nan_to_num(123.0), same.nan_to_num(123.0))
+    hk, hv = K.held(_np(k), bits, NAME[dtype]), K.held(_np(v), bits, NAME[dtype])
+    want, size = K.attention(_np(q), hk, hv, mask, dim ** -0.5)
+    got = _np(out[:2, :, 0]).reshape(2, n, 2 * group, dim)
+    nan = np.isnan(want)
+    assert np.array_equal(np.isnan(got), nan) and nan.any() == poisoned
+    bound = _bound(_np(q), hk, hv, mask, dim ** -0.5, dtype, want, size)
+    assert (np.abs(np.where(nan, 0, got - want)) <= np.where(nan, 0, bound)).all()
+
+
+@pytest.mark.parametrize("dtype,bits,dim", [(torch.bfloat16, 4, 128), (torch.float16, 8, 64)])
+def test_large_packed_and_shifted_launches(dtype, bits, dim):
+    """Packed rows of different counts with cache rows in place: the same bits as every sequence by itself at
+    its full length and unshifted, and rows behind the last one as they were."""
+    from recurrent_drafting_amd import attention, kv_cache
+    from recurrent_drafting_amd.packed_rows import PackedRows
+
+    rng = np.random.default_rng(53)
+    batch, heads, n, prev = 8, 32, 240, 250
+    counts = [240, 1, 33, 128, 129, 240, 31, 200]
+    rows = PackedRows.from_counts(torch.tensor(counts, dtype=torch.int32).cuda(), sum(counts), n)
+    k, v = (torch.tensor(rng.standard_normal((batch, heads, prev + n, dim))).to(dtype) for _ in range(2))
+    q = torch.tensor(rng.standard_normal((batch, heads, n, dim))).to(dtype).cuda()
+    pads = [0, 100, 40, 0, 64, 7, 200, 33]
+    mask = torch.tensor(_tree_mask(rng, batch, n, prev, pads)).cuda()
+    plain = _new(batch, prev + n, heads, dim, dtype, bits)
+    for view, x in zip(plain.sliced[0], (k, v)):
+        view.append(x.cuda())
+    want = attention.masked_attention(q, plain.sliced[0][0].rows(), plain.sliced[0][1].rows(),
+                                      attention.prepare(mask, n_heads=heads)).view(batch, n, heads, dim)
+    # cache row = column - shift
+    shift = torch.tensor([0, 100, 37, -1, 64, 7, 31, -2], dtype=torch.int32)
+    moved = _new(batch, prev + n + 2, heads, dim, dtype, bits)
+    moved._cache.fill_(0xFF)
+    for b in range(batch):
+        s = int(shift[b])
+        lo = max(s, 0)
+        moved._cache[0, :, b, :, lo - s : prev + n - s] = plain._cache[0, :, b, :, lo:]
+    moved.set_length(prev + n)
+    moved.rows_in_place = True
+    moved.shift.copy_(shift)
+    prepared = attention.prepare(mask, n_heads=heads, kv_shift=moved.shift)
+    packed = torch.cat([q[b, :, :c] for b, c in enumerate(counts)], dim=1).transpose(0, 1)
+    packed = torch.cat((packed, packed.new_full((rows.rows - sum(counts), heads, dim), float("nan"))))
+    key, value = (kv_cache.QuantizedRows(moved, 0, side, 0, prev + n) for side in (0, 1))
+    got = attention.masked_attention(packed, key, value, prepared, rows=rows).view(rows.rows, heads, dim)
+    at = 0
+    for b, c in enumerate(counts):
+        assert torch.equal(got[at : at + c], want[b, :c]), b
+        at += c
+
 
 # ---- packed rows, rows in place, moves ------------------------------------------------------------------
 
