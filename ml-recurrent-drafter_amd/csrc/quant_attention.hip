@@ -66,6 +66,7 @@ struct QuantArgs {
   int64_t max_len;
   int B, H, Hkv, group, n_q, kv_len, words, D, bits_per_code;
   int span_blocks, max_pieces, piece;
+  int sorted;      // workgroups take their tiles by rank (sorted_pair)
   float scale;     // softmax scale; times log2 e for the MFMA kernel
   float inv_scale; // its reciprocal
 };
@@ -192,6 +193,46 @@ __device__ inline void tile_keys(const QuantArgs& a, int b, int row0, int rows_p
   t.begin = t.lo / kUnit * kUnit;
   t.n_pieces = t.hi > t.lo ? (t.hi - t.begin + a.piece - 1) / a.piece : 1;
 }
+// The (batch row, tile) pair of a workgroup's place in the launch, the pairs with the most keys first: every thread
+// weighs one pair, and the one whose rank is the place is taken.  `weights` and `pick` are LDS.
+constexpr int kMaxSorted = 512;                     // pairs, one per thread of the widest workgroup
+__device__ inline int sorted_pair(const QuantArgs& a, int pairs, int tiles, int rows_per_tile, int place, uint32_t* weights, int* pick) {
+  const int tid = threadIdx.x;
+  uint32_t mine = 0;
+  if (tid < pairs) {
+    Tile t;
+    const int b = tid / tiles, row0 = tid % tiles * rows_per_tile;
+    tile_rows(a, b, t);
+    int lo = a.kv_len, hi = 0;
+    if (row0 < t.rows) {
+      const int end = row0 + rows_per_tile < t.rows ? row0 + rows_per_tile : t.rows;
+      const int s1 = (end - 1) / a.group / kSpanQueries;
+      const int4* const sp = reinterpret_cast<const int4*>(a.spans) + (int64_t)b * a.span_blocks;
+      for (int s0 = row0 / a.group / kSpanQueries; s0 <= s1; s0 += 8) {
+        int4 x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = sp[min(s0 + i, s1)];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) { lo = min(lo, x[i].x); hi = max(hi, x[i].y); }
+      }
+    }
+    // (no two are equal: the thread's number is in the low bits, the later tile first)
+    mine = (uint32_t)((hi > lo ? (hi - lo + kUnit - 1) / kUnit : 0) * kMaxSorted + tid);
+  }
+  weights[tid] = mine;
+  __syncthreads();
+  if (tid < pairs) {
+    int rank = 0;
+    for (int i = 0; i < pairs; i += 4) {            // (behind the last pair: zeros)
+      const u32x4 w = *reinterpret_cast<const u32x4*>(weights + i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) rank += w[e] > mine;
+    }
+    if (rank == place) *pick = tid;
+  }
+  __syncthreads();
+  return __builtin_amdgcn_readfirstlane(*pick);
+}
 __device__ inline Tile tile_of(const QuantArgs& a, int b, int row0, int rows_per_tile) {
   Tile t;
   tile_rows(a, b, t);
@@ -249,8 +290,18 @@ __global__ __launch_bounds__(R * K * 64, 2) void attn_quant_kernel(QuantArgs a) 
   float* const s_o = reinterpret_cast<float*>(s_mem);
 
   // (a causal prompt's last rows have the most keys: first)
-  const int hk = blockIdx.x % a.Hkv, tile = gridDim.x / a.Hkv - 1 - blockIdx.x / a.Hkv;
-  const int b = blockIdx.y / a.max_pieces, piece = blockIdx.y % a.max_pieces;
+  const int tiles = gridDim.x / a.Hkv, hk = blockIdx.x % a.Hkv;
+  int tile = tiles - 1 - blockIdx.x / a.Hkv;
+  int b = blockIdx.y / a.max_pieces;
+  const int piece = blockIdx.y % a.max_pieces;
+  if constexpr (R > 1) {
+    if (a.sorted) {
+      __shared__ int s_pick;
+      const int pair = sorted_pair(a, a.B * tiles, tiles, kRows, blockIdx.y * tiles + blockIdx.x / a.Hkv,
+                                   reinterpret_cast<uint32_t*>(s_mem), &s_pick);
+      b = pair / tiles; tile = pair % tiles;
+    }
+  }
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, grp = lane >> 4;
@@ -1040,7 +1091,7 @@ constexpr int kComputeUnits = 256;
 // The launch of a shape: the workgroup's layout (see attn_quant_kernel) and how the keys are cut.
 enum Layout { kNarrow, kMiddle2, kMiddle4, kWide };
 constexpr int kTileRows[] = {16, 32, 32, 256}, kLayoutWaves[] = {8, 2, 4, 8};
-struct Shape { int layout, tile_rows, tiles, piece, max_pieces; };
+struct Shape { int layout, tile_rows, tiles, piece, max_pieces, sorted; };
 Shape shape_of(int batch, int n_heads, int n_kv_heads, int n_q, int kv_len) {
   Shape s;
   const int64_t rows = (int64_t)n_q * (n_heads / n_kv_heads), slabs = (int64_t)batch * n_kv_heads;
@@ -1060,6 +1111,10 @@ Shape shape_of(int batch, int n_heads, int n_kv_heads, int n_q, int kv_len) {
   else s.layout = blocks >= 4 * kComputeUnits ? kMiddle2 : kMiddle4;
   s.tile_rows = kTileRows[s.layout];
   s.tiles = (int)rd::ceil_div(rows, s.tile_rows);
+  // A prompt's large tiles, longest first whatever the mask: its last rows have the most keys, and so have the rows
+  // of left padding, which attend to everything where the model asks for that (batch 2, 1900 tokens, such padding:
+  // 133 -> 96 us; without padding 2.5 us more than in the order of the rows).
+  s.sorted = s.layout == kWide && prompt && (int64_t)batch * s.tiles <= kMaxSorted;
   // Keys are cut into pieces as far as every SIMD needs waves: two with few rows, where the kernel waits for
   // memory (one sequence of 65 536 keys in 8 bits, 8 kv heads: 35 against 44 us), one otherwise (batch 8, 32
   // heads, 20 rows, 1000 keys: 25 against 30 us).  A piece has at least two (four) units per wave, and a cut
@@ -1161,6 +1216,7 @@ extern "C" int rd_verify_attention_quant(const void* q, const int64_t* q_strides
   a.B = batch; a.H = n_heads; a.Hkv = n_kv_heads; a.group = n_heads / n_kv_heads; a.n_q = n_q; a.kv_len = kv_len;
   a.words = (kv_len + 63) / 64; a.D = head_dim; a.bits_per_code = bits;
   a.span_blocks = (int)rd::ceil_div(n_q, kSpanQueries);
+  a.sorted = 0;
   a.max_pieces = 1; a.piece = (int)(rd::ceil_div((int64_t)kv_len + kUnit - 1, kUnit) * kUnit);
   a.scale = scale; a.inv_scale = 1.f;
   hipStream_t s = rd::as_stream(stream);
@@ -1171,6 +1227,7 @@ extern "C" int rd_verify_attention_quant(const void* q, const int64_t* q_strides
     RD_REQUIRE((int64_t)batch * sh.max_pieces <= 65535 && (int64_t)n_kv_heads * sh.tiles <= 2147483647LL, RD_ELIMIT,
                "%s: grid too large", who);
     a.max_pieces = sh.max_pieces; a.piece = sh.piece;
+    a.sorted = sh.sorted;
     a.scale = scale * 1.4426950408889634f;
     a.inv_scale = 1.f / a.scale;
     if (sh.max_pieces > 1) {
