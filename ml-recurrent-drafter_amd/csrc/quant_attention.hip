@@ -255,7 +255,10 @@ __device__ inline float row_max(float v) {
 // MFMA kernel
 // ---------------------------------------------------------------------------------------------
 template <typename T, int BITS, int D, int RB, int R, int K>
-__global__ __launch_bounds__(R * K * 64, 2) void attn_quant_kernel(QuantArgs a) {
+// (Three waves on a SIMD where head_dim is 64 and R is 1, though 20 to 56 bytes of registers go to scratch for it: batch
+// 16, 32 / 8 heads, 46 rows, 1257 keys 24.2 -> 20.3 us, 40 heads, 162 rows, 1962 keys in 8 bits 99 -> 88 us.  At 128 the
+// third wave would put most of the accumulators there.)
+__global__ __launch_bounds__(R * K * 64, D == 64 && R == 1 ? 3 : 2) void attn_quant_kernel(QuantArgs a) {
   static_assert(R == 1 || K == 1, "waves side by side or behind each other");
   using O = Ops<T>;
   constexpr int kRec = record_bytes(BITS, D), kCodes = code_bytes(BITS, D);
@@ -1092,7 +1095,7 @@ constexpr int kComputeUnits = 256;
 enum Layout { kNarrow, kMiddle2, kMiddle4, kWide };
 constexpr int kTileRows[] = {16, 32, 32, 256}, kLayoutWaves[] = {8, 2, 4, 8};
 struct Shape { int layout, tile_rows, tiles, piece, max_pieces, sorted; };
-Shape shape_of(int batch, int n_heads, int n_kv_heads, int n_q, int kv_len) {
+Shape shape_of(int batch, int n_heads, int n_kv_heads, int n_q, int kv_len, int head_dim) {
   Shape s;
   const int64_t rows = (int64_t)n_q * (n_heads / n_kv_heads), slabs = (int64_t)batch * n_kv_heads;
   // kWide converts a unit once for 256 rows, in one workgroup of eight waves on a compute unit.  It is the faster
@@ -1102,12 +1105,16 @@ Shape shape_of(int batch, int n_heads, int n_kv_heads, int n_q, int kv_len) {
   // against 50 us.  Prompts wait for the longest of their tiles, which the first round has; they need a quarter of a
   // round more: batch 2, 32 / 8 heads, 1300 tokens (1.3 rounds) 55 against 62 us, batch 1, 2000 tokens (1 round) 75
   // against 61 us.
+  // At head_dim 64, where the other layouts have three waves on a SIMD, it takes 7/8 (batch 8, 32 heads, 1200 keys: 200
+  // rows 38 against 48 us, 400 rows (0.81) 72 against 67 us) and half a round (batch 1, 32 / 8 heads, 2500 tokens (1.25)
+  // 63 against 57 us; batch 2, 1900 tokens (1.9) 60 against 65 us).
   // Two waves per tile where that alone gives every SIMD two waves (34 against 37 us), else four (batch 8,
   // 32 heads, 48 rows, 1000 keys: 27 against 34 us).
   const int64_t wide = slabs * rd::ceil_div(rows, 256), blocks = slabs * rd::ceil_div(rows, 32);
   const bool prompt = n_q > kv_len / 2;
   if (rows <= 16) s.layout = kNarrow;
-  else if (prompt ? 4 * wide >= 5 * kComputeUnits : 4 * blocks >= 3 * 8 * kComputeUnits * rd::ceil_div(wide, kComputeUnits)) s.layout = kWide;
+  else if (prompt ? 4 * wide >= (head_dim == 64 ? 6 : 5) * kComputeUnits
+                  : blocks >= (head_dim == 64 ? 7 : 6) * kComputeUnits * rd::ceil_div(wide, kComputeUnits)) s.layout = kWide;
   else s.layout = blocks >= 4 * kComputeUnits ? kMiddle2 : kMiddle4;
   s.tile_rows = kTileRows[s.layout];
   s.tiles = (int)rd::ceil_div(rows, s.tile_rows);
@@ -1173,7 +1180,7 @@ extern "C" size_t rd_verify_attention_quant_workspace_bytes(int dtype, int batch
                                                             int kv_len, int head_dim) {
   if (batch <= 0 || n_heads <= 0 || n_kv_heads <= 0 || n_q <= 0 || kv_len <= 0 || n_heads % n_kv_heads != 0 ||
       !mfma_shape(dtype, head_dim)) return 0;
-  const Shape s = shape_of(batch, n_heads, n_kv_heads, n_q, kv_len);
+  const Shape s = shape_of(batch, n_heads, n_kv_heads, n_q, kv_len, head_dim);
   if (s.max_pieces == 1) return 0;
   const size_t rows = (size_t)batch * s.max_pieces * n_heads * n_q;
   return rd::align_up(rows * head_dim * sizeof(float), 256) + rd::align_up(rows * 2 * sizeof(float), 256);
@@ -1223,7 +1230,7 @@ extern "C" int rd_verify_attention_quant(const void* q, const int64_t* q_strides
   auto whole = [](const int64_t* st, int m) { return st[0] % m == 0 && st[1] % m == 0 && st[2] % m == 0; };
   const bool mfma = !force_generic && mfma_shape(dtype, head_dim) && al(q, 16) && al(out, 8) && whole(q_strides, 8) && whole(o_strides, 4);
   if (mfma) {
-    const Shape sh = shape_of(batch, n_heads, n_kv_heads, n_q, kv_len);
+    const Shape sh = shape_of(batch, n_heads, n_kv_heads, n_q, kv_len, head_dim);
     RD_REQUIRE((int64_t)batch * sh.max_pieces <= 65535 && (int64_t)n_kv_heads * sh.tiles <= 2147483647LL, RD_ELIMIT,
                "%s: grid too large", who);
     a.max_pieces = sh.max_pieces; a.piece = sh.piece;

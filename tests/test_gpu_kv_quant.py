@@ -400,7 +400,8 @@ def _repeated(q, k, v, batch, copies, dtype, bits):
 
 LARGE = [  # batch, kv heads, group, n_q, prev, mask
     (8, 24, 1, 230, 300, "tree"), (13, 16, 2, 121, 133, "tree"), (10, 8, 4, 225, 0, "causal"), (8, 32, 1, 115, 150, "tree"),
-    (16, 20, 1, 250, 20, "causal"), (9, 64, 1, 255, 260, "scattered")]
+    (16, 20, 1, 250, 20, "causal"), (9, 64, 1, 255, 260, "scattered"),
+    (8, 32, 1, 250, 260, "tree"), (12, 16, 2, 225, 0, "causal")]
 
 
 @pytest.mark.parametrize("dtype,bits,dim", [(torch.bfloat16, 4, 128), (torch.float16, 8, 64), (torch.bfloat16, 8, 128), (torch.float16, 4, 64)])
