@@ -419,9 +419,10 @@ RD_API int rd_rope_verify_attention(const void* q, const int64_t* q_strides, con
  * written from; rows start on 16-byte boundaries of `out`).
  *
  * rd_verify_attention_quant: rd_verify_attention over such rows; mask bits, plan and row_start as
- * there.  spans: rd_attn_spans_ints(batch, n_q) int32 written by rd_attn_spans from the mask bits (once
- * per forward: the first and one past the last key that 16 consecutive queries attend to).  A row that
- * attends to nothing is written as zeros; keys nobody attends to may hold NaN blocks.  bf16 and fp16
+ * there.  spans: rd_attn_spans_ints(batch, n_q) int32, 16-byte aligned, written by rd_attn_spans from the
+ * mask bits once per forward (for every 16 consecutive queries: the first and one past the last key that
+ * one of them attends to, and a run of keys that all of them attend to).  A row that attends to nothing
+ * is written as zeros; keys nobody attends to may hold NaN blocks.  bf16 and fp16
  * with head_dim 64 or 128 (q 16-byte aligned with strides that are multiples of 8 elements, out 8-byte
  * aligned with strides that are multiples of 4) run on the MFMA kernel, everything else, or
  * force_generic != 0, on the generic kernel.  workspace: rd_verify_attention_quant_workspace_bytes (0:
@@ -447,6 +448,9 @@ RD_API int rd_kv_dequantize(const void* cache, const int64_t* cache_strides, int
 RD_API size_t rd_attn_spans_ints(int batch, int n_q);
 RD_API int rd_attn_spans(const uint64_t* bits, int batch, int n_q, int kv_len, int32_t* spans,
                          void* stream);
+/* A number that the capture going on on `stream` has to itself, 0 if there is none: what a captured
+ * kernel has written may be read by the same capture only. */
+RD_API uint64_t rd_stream_capture_id(void* stream);
 RD_API size_t rd_verify_attention_quant_workspace_bytes(int dtype, int batch, int n_heads,
                                                         int n_kv_heads, int n_q, int kv_len,
                                                         int head_dim);

@@ -1176,6 +1176,14 @@ extern "C" int rd_attn_spans(const uint64_t* bits, int batch, int n_q, int kv_le
   return rd::check_launch("rd_attn_spans");
 }
 
+extern "C" uint64_t rd_stream_capture_id(void* stream) {
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  // (the null stream is never captured, and asking it during another stream's capture is an error)
+  if (stream == nullptr || hipStreamGetCaptureInfo(rd::as_stream(stream), &status, &id) != hipSuccess) return 0;
+  return status == hipStreamCaptureStatusActive ? id + 1 : 0;
+}
+
 extern "C" size_t rd_verify_attention_quant_workspace_bytes(int dtype, int batch, int n_heads, int n_kv_heads, int n_q,
                                                             int kv_len, int head_dim) {
   if (batch <= 0 || n_heads <= 0 || n_kv_heads <= 0 || n_q <= 0 || kv_len <= 0 || n_heads % n_kv_heads != 0 ||

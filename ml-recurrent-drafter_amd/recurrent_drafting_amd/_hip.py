@@ -81,6 +81,7 @@ _PROTOTYPES = {
     "rd_kv_dequantize": (_I, [_P, _P, _I, _I, _I, _I, _L, _L, _I, _L, _P, _P, _P]),
     "rd_attn_spans_ints": (_Z, [_I, _I]),
     "rd_attn_spans": (_I, [_P, _I, _I, _I, _P, _P]),
+    "rd_stream_capture_id": (C.c_uint64, [_P]),
     "rd_verify_attention_quant_workspace_bytes": (_Z, [_I, _I, _I, _I, _I, _I, _I]),
     "rd_verify_attention_quant": (
         _I,

@@ -61,8 +61,8 @@ class PreparedMask:
     kv_len: int
     workspace: Optional[torch.Tensor] = None
     shifted: bool = False  # the plan was built with per-row cache shifts (kv_cache.Cache.shift)
-    # first and one past the last key that 16 consecutive queries attend to: made by the first attention
-    # over a cache in 4 or 8 bits that uses this mask, per stream ({stream handle: int32 tensor})
+    # which keys 16 consecutive queries attend to, as rd_attn_spans writes it: made by the first attention over
+    # a cache in 4 or 8 bits that uses this mask, per stream ({stream handle, or (handle, capture): int32 tensor})
     spans: dict = field(default_factory=dict)
 
 
@@ -161,17 +161,21 @@ def masked_attention(
 
 def _spans(prepared: PreparedMask) -> torch.Tensor:
     """The mask's span table, written on the current stream: kept for the later layers on that stream.
-    A table written while a graph is captured holds nothing before the replay, so it stays with its call."""
+    A table written while a graph is captured holds nothing before the replay: it is for the layers of that
+    capture."""
     stream = _hip.stream()
     spans = prepared.spans.get(stream)
     if spans is None:
         lib = _hip.lib()
+        capture = lib.rd_stream_capture_id(stream)
+        key = (stream, capture) if capture else stream
+        spans = prepared.spans.get(key)
+    if spans is None:
         spans = torch.empty(lib.rd_attn_spans_ints(prepared.batch, prepared.n_q), dtype=torch.int32,
                             device=prepared.bits.device)
         _hip.check(lib.rd_attn_spans(_hip.ptr(prepared.bits), prepared.batch, prepared.n_q, prepared.kv_len,
                                      _hip.ptr(spans), stream))
-        if not torch.cuda.is_current_stream_capturing():
-            prepared.spans[stream] = spans
+        prepared.spans[key] = spans
     return spans
 
 
@@ -188,6 +192,7 @@ def _quantized_attention(q, k, v, prepared: PreparedMask, scale, force_generic, 
         B, n_q = rows.batch, rows.n
         assert T == rows.rows
     assert (Bk, D) == (B, Dq) and (v._prev, v._length) == (k._prev, k._length)
+    assert k._prev == 0 or not prepared.shifted, "shifted cache rows are counted from the cache's first row"
     assert q.dtype == owner.dtype, "queries in the type the cache was written from"
     assert (prepared.batch, prepared.n_q, prepared.kv_len) == (B, n_q, kv_len), "mask/plan mismatch"
     _hip.on_current_device(q, owner._cache, prepared.bits)

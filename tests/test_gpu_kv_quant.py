@@ -671,6 +671,43 @@ def test_side_stream_graphs_and_shared_masks():
     assert torch.equal(outs[0][0], want[2]) and torch.equal(outs[1][0], want[3])
 
 
+def test_a_captured_forward_follows_its_mask():
+    """The mask is prepared inside the capture: its span table is written once for the layers of the capture,
+    again by every replay, and is not what an eager call on the same stream reads afterwards."""
+    from recurrent_drafting_amd import attention
+
+    rng = np.random.default_rng(59)
+    kv, n = 300, 20
+    cache = _new(2, kv, 2, 64, torch.float16, 8, layers=3)
+    for views in cache.sliced:
+        for view in views:
+            view.append(torch.tensor(rng.standard_normal((2, 2, kv, 64))).half().cuda())
+    q = torch.randn(2, 4, n, 64, device="cuda").half()
+    masks = [torch.tensor(_tree_mask(rng, 2, n, kv - n, pads)).cuda() for pads in ([0, 90], [200, 0], [33, 250])]
+
+    def forward(mask):
+        prepared = attention.prepare(mask, n_heads=4)
+        return prepared, [attention.masked_attention(q, k.rows(), v.rows(), prepared) for k, v in cache.sliced]
+
+    want = [[o.clone() for o in forward(m)[1]] for m in masks]
+    static, stream = masks[0].clone(), torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        prepared, outs = forward(static)
+    assert len(prepared.spans) == 1 and all(isinstance(key, tuple) for key in prepared.spans)
+    for turn in (1, 2, 0, 1):
+        static.copy_(masks[turn])
+        graph.replay()
+        eager = forward(masks[2])[1]
+        torch.cuda.synchronize()
+        for i in range(3):
+            assert torch.equal(outs[i], want[turn][i]) and torch.equal(eager[i], want[2][i])
+    with torch.cuda.stream(stream):
+        again = attention.masked_attention(q, cache.sliced[1][0].rows(), cache.sliced[1][1].rows(), prepared)
+    stream.synchronize()
+    assert torch.equal(again, want[1][1]) and len(prepared.spans) == 2
+
+
 def test_same_call_twice_gives_the_same_bits():
     from recurrent_drafting_amd import attention
 
@@ -700,6 +737,10 @@ def test_refusals_with_tensors():
         attention.masked_attention(q.half(), key.rows(), value.rows(), prepared)
     with pytest.raises(AssertionError):
         attention.masked_attention(q, key.rows(1), value.rows(1), prepared)
+    shifted = attention.prepare(torch.ones(1, 1, 19, dtype=torch.bool, device="cuda"), n_heads=4,
+                                kv_shift=torch.zeros(1, dtype=torch.int32, device="cuda"))
+    with pytest.raises(AssertionError, match="first row"):  # a shift could point in front of the slice
+        attention.masked_attention(q, key.rows(1), value.rows(1), shifted)
     with pytest.raises(RuntimeError, match="scale"):
         attention.masked_attention(q, key.rows(), value.rows(), prepared, scale=-0.5)
     x = torch.zeros(1, 1, 4 * 64, dtype=torch.bfloat16, device="cuda")

@@ -27,6 +27,10 @@ def test_row_bytes():
         assert lib.rd_kv_quant_row_bytes(bits, dim) == want
 
 
+def test_nothing_is_captured_on_the_null_stream():
+    assert _lib().rd_stream_capture_id(None) == 0
+
+
 def _append(lib, batch=2, n_new=3, heads=4, kv_heads=2, dim=64, bits=4, row0=0, max_len=8, dtype=BF16, table=16,
             q=FAKE, strides=(256 * 3, 256), cache=(48 * 8 * 2, 48 * 8, 48), k_cache=FAKE):
     return lib.rd_rope_append_quant(q, _s(*strides), FAKE, _s(*strides), FAKE, _s(*strides), dtype, batch, n_new, heads,
@@ -84,6 +88,7 @@ def _attend(lib, batch=2, heads=8, kv_heads=2, n_q=3, kv=100, dim=128, bits=4, d
     (dict(dtype=9), EINVAL, b"dtype"), (dict(bits=6), EINVAL, b"bits"), (dict(dim=80), ELIMIT, b"multiple of 32"),
     (dict(batch=65536), ELIMIT, b"65535"), (dict(kv=2 ** 23 + 1), ELIMIT, b"2^23"), (dict(n_q=2 ** 29), ELIMIT, b"query rows"),
     (dict(q=None), EINVAL, b"null"), (dict(spans=None), EINVAL, b"null"), (dict(max_len=0), EINVAL, b"empty"),
+    (dict(spans=FAKE + 4), EINVAL, b"aligned"),
     (dict(scale=0.0), EINVAL, b"scale"), (dict(scale=-1.0), EINVAL, b"scale"), (dict(scale=float("nan")), EINVAL, b"scale"),
     (dict(scale=float("inf")), EINVAL, b"scale"), (dict(cache=FAKE + 8), EINVAL, b"aligned"),
     (dict(cs=(80 * 512, 80 * 256, 96)), EINVAL, b"strides"), (dict(cs=(80 * 512 + 4, 80 * 256, 80)), EINVAL, b"strides"),
