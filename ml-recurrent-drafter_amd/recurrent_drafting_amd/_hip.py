@@ -183,12 +183,10 @@ I64x2, I64x3 = C.c_int64 * 2, C.c_int64 * 3  # stride arguments
 
 def on_current_device(*tensors: torch.Tensor) -> None:
     """Refuses tensors that are not on the current GPU: launches go to its current stream."""
-    for t in tensors:
-        if t.get_device() < 0:
-            ptr(t)  # says what it thinks of host tensors
     current = _raw_device() if _raw_device is not None else torch.cuda.current_device()
     for t in tensors:
         if t.get_device() != current:
+            ptr(t)  # says what it thinks of host tensors
             raise RuntimeError(f"tensor on {t.device}, but the current GPU is cuda:{current}: "
                                "make the tensors' GPU the current one (torch.cuda.device)")
 

@@ -159,11 +159,10 @@ def masked_attention(
     return out.view(B, n_q, H * D) if rows is None else out.view(rows.rows, H * D)
 
 
-def _spans(prepared: PreparedMask) -> torch.Tensor:
-    """The mask's span table, written on the current stream: kept for the later layers on that stream.
+def _spans(prepared: PreparedMask, stream: int) -> torch.Tensor:
+    """The mask's span table, written on `stream`, the current one: kept for the later layers on that stream.
     A table written while a graph is captured holds nothing before the replay: it is for the layers of that
     capture."""
-    stream = _hip.stream()
     spans = prepared.spans.get(stream)
     if spans is None:
         lib = _hip.lib()
@@ -183,18 +182,19 @@ def _quantized_attention(q, k, v, prepared: PreparedMask, scale, force_generic, 
     """masked_attention over the rows of a cache in 4 or 8 bits (rd_verify_attention_quant)."""
     assert isinstance(k, kv_cache.QuantizedRows) and isinstance(v, kv_cache.QuantizedRows) and \
         k._owner is v._owner, "keys and values of one cache"
-    owner = k._owner
-    Bk, Hkv, kv_len, D = k.shape
+    owner, prev = k._owner, k._prev
+    Bk, Hkv, max_len = owner.slab_shape
+    kv_len, D = k._length - prev, owner.head_dim
     if rows is None:
         B, H, n_q, Dq = q.shape
     else:
         T, H, Dq = q.shape
         B, n_q = rows.batch, rows.n
         assert T == rows.rows
-    assert (Bk, D) == (B, Dq) and (v._prev, v._length) == (k._prev, k._length)
-    assert k._prev == 0 or not prepared.shifted, "shifted cache rows are counted from the cache's first row"
+    assert Bk == B and D == Dq and v._prev == prev and v._length == k._length
+    assert prev == 0 or not prepared.shifted, "shifted cache rows are counted from the cache's first row"
     assert q.dtype == owner.dtype, "queries in the type the cache was written from"
-    assert (prepared.batch, prepared.n_q, prepared.kv_len) == (B, n_q, kv_len), "mask/plan mismatch"
+    assert prepared.batch == B and prepared.n_q == n_q and prepared.kv_len == kv_len, "mask/plan mismatch"
     _hip.on_current_device(q, owner._cache, prepared.bits)
     if q.stride(-1) != 1:
         q = q.contiguous()
@@ -207,8 +207,8 @@ def _quantized_attention(q, k, v, prepared: PreparedMask, scale, force_generic, 
         out = q.new_empty((rows.rows, width))
         q_strides = _hip.I64x3(0, q.stride(1), q.stride(0))
         o_strides = _hip.I64x3(0, D, width)
-    lib = _hip.lib()
-    spans = _spans(prepared)
+    lib, stream = _hip.lib(), _hip.stream()
+    spans = _spans(prepared, stream)
     # partial results of keys cut into pieces: memory of this call alone, so that calls on several
     # streams, or captured in several graphs, may share the mask
     ws_bytes = lib.rd_verify_attention_quant_workspace_bytes(owner.dtype_code, B, H, Hkv, n_q, kv_len, D)
@@ -218,10 +218,10 @@ def _quantized_attention(q, k, v, prepared: PreparedMask, scale, force_generic, 
     _hip.check(
         lib.rd_verify_attention_quant(
             q.data_ptr(), q_strides, k.data_ptr(), v.data_ptr(), owner.byte_strides, owner.bits,
-            owner._cache.shape[4] - k._prev, out.data_ptr(), o_strides, owner.dtype_code, B, H, Hkv, n_q, kv_len, D,
+            max_len - prev, out.data_ptr(), o_strides, owner.dtype_code, B, H, Hkv, n_q, kv_len, D,
             1.0 / math.sqrt(D) if scale is None else float(scale), prepared.bits.data_ptr(), prepared.plan.data_ptr(),
             spans.data_ptr(), workspace.data_ptr() if ws_bytes else None, ws_bytes, int(force_generic),
-            _hip.ptr(rows.row_start) if rows is not None else None, _hip.stream(),
+            _hip.ptr(rows.row_start) if rows is not None else None, stream,
         )
     )
     return out

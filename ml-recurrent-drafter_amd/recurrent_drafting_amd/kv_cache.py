@@ -53,8 +53,9 @@ class QuantizedRows:
 
     @property
     def shape(self) -> Tuple[int, int, int, int]:
-        _, _, batch, n_heads, _, _ = self._owner._cache.shape
-        return (batch, n_heads, self._length - self._prev, self._owner.head_dim)
+        owner = self._owner
+        batch, n_heads, _ = owner.slab_shape
+        return (batch, n_heads, self._length - self._prev, owner.head_dim)
 
     @property
     def records(self) -> torch.Tensor:
@@ -225,7 +226,7 @@ def _rope_append_quantized(q, k, v, cos, sin, position_ids, key_view: View, valu
     """rope_append into a cache in 4 or 8 bits (rd_rope_append_quant).  For a single token the kernel takes less
     time than this function, so every tensor is asked once for what is needed of it."""
     cache, owner, layer, length = key_view._cache, key_view._owner, key_view._layer, key_view.length
-    _, _, batch, n_kv_heads, max_length, _ = cache.shape
+    batch, n_kv_heads, max_length = owner.slab_shape
     head_dim = owner.head_dim
     q_shape, k_shape, q_stride, k_stride, v_stride = q.shape, k.shape, q.stride(), k.stride(), v.stride()
     width, kv_width = q_shape[-1], n_kv_heads * head_dim
@@ -257,11 +258,12 @@ def _rope_append_quantized(q, k, v, cos, sin, position_ids, key_view: View, valu
         out_strides = _hip.I64x2(0, width)
     keys = QuantizedRows(owner, layer, 0, 0, length + n_new)
     values = QuantizedRows(owner, layer, 1, 0, length + n_new)
+    first = keys.data_ptr()
     _hip.check(
         _hip.lib().rd_rope_append_quant(
             q.data_ptr(), q_strides, k.data_ptr(), k_strides, v.data_ptr(), v_strides, owner.dtype_code, batch, n_new,
             n_heads, n_kv_heads, head_dim, cos.data_ptr(), sin.data_ptr(), table[0], position_ids.data_ptr(),
-            positions[0], q_out.data_ptr(), out_strides, keys.data_ptr(), values.data_ptr(), owner.byte_strides,
+            positions[0], q_out.data_ptr(), out_strides, first, first + owner.slab_strides[1], owner.byte_strides,
             owner.bits, length, max_length, None if rows is None else _hip.ptr(rows.row_start),
             _hip.ptr(owner.shift) if owner._rows_in_place else None, _hip.stream(),
         )
@@ -300,6 +302,7 @@ class Cache:
         if bits is not None:
             layer, kv, batch, head, row, _ = self._cache.stride()
             self.byte_strides = _hip.I64x3(batch, head, row)
+            self.slab_shape = (batch_size, n_heads, max_length)
             self.slab_strides = (layer, kv, row)  # bytes from layer to layer, from keys to values, from row to row
         self.sliced = tuple(
             (View(self._cache, layer, 0, self), View(self._cache, layer, 1, self)) for layer in range(n_layers)
