@@ -7,13 +7,9 @@
 //   attn_quant_kernel    bf16 and fp16, head_dim 64 and 128, on v_mfma_f32_16x16x32
 //   attn_quant_generic_kernel  every other type and head size the cache has
 //
-// attn_quant_kernel.  The query heads of a kv head are folded into the rows (row = query * group +
-// head in group), so that K and V are read once per kv head.  A workgroup owns 16 * RB * R rows and a
-// piece of the keys: R waves side by side take 16 * RB rows each, K waves behind each other take the 32-key
-// units of the piece in turn, each with a running maximum, sum and accumulators of its own, merged through
-// LDS at the end.  Records travel memory -> registers (whole contiguous units, 16 bytes per lane) -> LDS as
-// they lie in memory; the operands of the matrix instructions are read from there without a bank conflict
-// (rows of 48, 80 and 144 bytes spread 16 lanes over all banks), codes become 16-bit numbers in registers.
+// attn_quant_kernel.  The query heads of a kv head are folded into the rows (row = query * group + head in
+// group), so that K and V are read once per kv head.  A wave takes 16 * RB rows and goes over units of 32 keys
+// with a running maximum, row sums and accumulators in registers:
 //   S^T = K Q^T  A operand: lane (key l % 16, chunk l / 16) needs 8 consecutive k-slots per step.  The
 //                order of the dims in a dot product is free, so chunk c of the record is dims
 //                [c D/4, (c+1) D/4): D/4 contiguous codes per lane, one block of 8 per step.
@@ -22,15 +18,43 @@
 //                whose scores the lane already holds (16 t + 4 (l / 16) + i), so P^T goes from the
 //                accumulators of the first product into the B operand of the second as it is.
 //                Codes of two keys become two dims times two keys: two conversions (code pair x scale
-//                to bf16, one instruction, exact) and two byte permutes.
-// A query row lives in one column of the accumulators (l % 16), so rescaling is a lane scalar; the
-// running maximum is lazy: raised only when some score exceeds it by 2^8, the row sum is kept per lane.
-// Keys outside the piece and outside the row's attended span read as zeros through the range check of
-// a buffer descriptor, without touching memory.
+//                to a 16-bit pair, one instruction, exact) and two byte permutes.
+// P is rounded to the 16-bit type there (half a step of it, 2^-9 or 2^-12 of a weight, as every 16-bit product
+// of the model rounds); scores, maximum, sums and accumulators are fp32.  The row sums come out of the
+// matrix pipeline too, as the product of P with ones: the sum of the rounded weights, the ones that V is
+// multiplied with.
+// A query row lives in one column of the accumulators (l % 16), so rescaling is a lane scalar; the running
+// maximum is lazy: raised only when some score exceeds it by 2^8 in the exponential, where fp32 has room
+// for 2^120 such weights.
 //
-// V and masked keys: a probability of zero does not silence a NaN in V (0 * NaN).  Blocks of V that read
-// back as NaN are taken out of the product, and the rows that attend to such a key get their NaN from a
-// second product of the mask with the marks of those blocks.
+// Records travel memory -> registers (whole contiguous units, 16 bytes per lane) -> LDS as they lie in
+// memory, and are picked apart from there without a bank conflict (rows of 48, 80 and 144 bytes spread 16
+// lanes over all banks): picked apart from memory, each unit took 22 scattered loads and the return path of
+// the vector memory was busy for 80 to 95 % of the time.  Keys outside the piece and outside the tile's
+// attended span read as zeros through the range check of a buffer descriptor, without touching memory.  Mask
+// words travel with their unit, and only where the span table does not say that every row attends to it.
+//
+// Four layouts (shape_of chooses, with both sides measured):
+//   rows <= 16      RB 1, eight waves behind each other take the units in turn and are merged through LDS.
+//                   Bound by memory: batch 8, 32 heads, one token, 2548 keys in 4 bits: 16 us, 4.4 TB/s of records
+//                   (a copy of 1 GiB reaches 5.15); one sequence of 65 537 keys in 8 bits, 8 kv heads: 29 to 32 us
+//                   and 4 for the merge of its pieces, 4.5 TB/s.
+//   <= 32 a tile    RB 2, two or four waves behind each other.  Bound by the vector ALU, which converts every unit
+//                   for 32 rows (about 130 of 230 instructions), and by the matrix pipeline, which runs beside it
+//                   for a small part of the time only: batch 8, 32 heads, a tree of 115 over 735 keys: 23 us, 390
+//                   TFLOP/s.
+//   <= 256 a tile   RB 2, eight waves side by side: a unit is converted once for all of them, its operands lie in LDS
+//                   in the lanes' order.  8 x 32 heads, 768 rows, 8192 keys: 898 us, 919 TFLOP/s in 4 bits, 854 us in
+//                   8 bits, where a large bf16 matrix product of the library reaches 1200; of the rest, conversion
+//                   costs about 100 ns of the 585 per unit and SIMD and the operands' way through LDS 60.
+// Tried and slower: 48 and 64 rows a wave (registers spill, or one wave on a SIMD: tree of 115 over 735 keys 38 us), two
+// and four waves side by side with two buffers (40 and 33 us), the next unit's first product put between the softmax's
+// instructions by hand (363 us where priorities gave 347), K's operands of the coming unit read as late as needed.
+//
+// V and masked keys: a probability of zero does not silence a NaN in V (0 * NaN).  Where the output of a
+// workgroup holds a NaN, its waves go over their keys once more: blocks of V that read back as NaN are then
+// taken out of the product, and the rows that attend to such a key get their NaN from a second product, of
+// the mask with the marks of those blocks.
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
 
@@ -255,7 +279,7 @@ __device__ inline float row_max(float v) {
 // MFMA kernel
 // ---------------------------------------------------------------------------------------------
 template <typename T, int BITS, int D, int RB, int R, int K>
-// (Three waves on a SIMD where head_dim is 64 and R is 1, though 20 to 56 bytes of registers go to scratch for it: batch
+// (Three waves on a SIMD where head_dim is 64 and R is 1, for which the second sweep keeps 20 to 56 bytes in scratch: batch
 // 16, 32 / 8 heads, 46 rows, 1257 keys 24.2 -> 20.3 us, 40 heads, 162 rows, 1962 keys in 8 bits 99 -> 88 us.  At 128 the
 // third wave would put most of the accumulators there.)
 __global__ __launch_bounds__(R * K * 64, D == 64 && R == 1 ? 3 : 2) void attn_quant_kernel(QuantArgs a) {
@@ -650,7 +674,7 @@ __global__ __launch_bounds__(R * K * 64, D == 64 && R == 1 ? 3 : 2) void attn_qu
         const VPairs pairs = v_pairs(c);
         if (i + kWaves < n_units) next(i + kWaves);
         __builtin_amdgcn_sched_barrier(0);
-        __builtin_amdgcn_s_setprio(1);             // (as below: 8 x 32 heads, 128 queries, 1000 keys: 36.6 -> 34.1 us)
+        __builtin_amdgcn_s_setprio(1);             // (as below: 8 x 32 heads, 128 queries, 1000 keys: 37.5 -> 35.0 us)
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) l[rb] = O::mfma(ones, pf[rb], l[rb]);
 #pragma unroll
@@ -702,7 +726,7 @@ __global__ __launch_bounds__(R * K * 64, D == 64 && R == 1 ? 3 : 2) void attn_qu
           for (int rb = 0; rb < RB; ++rb) sc[rb][0] = sc[rb][1] = f32x4{0.f, 0.f, 0.f, 0.f};
           // The wave in the matrix products goes before the one in the softmax on the same SIMD, whose
           // exponentials fill the gaps; with equal priorities the two tend to be in the same phase
-          // (16 x 32 heads, 128 queries, 8192 keys: 371 -> 347 us).
+          // (8 x 32 heads, 768 queries, 8192 keys: 941 -> 919 us, of 64 dims 551 -> 530).
           __builtin_amdgcn_s_setprio(1);
 #pragma unroll
           for (int s = 0; s < kSteps; ++s) {
@@ -770,7 +794,7 @@ __global__ __launch_bounds__(R * K * 64, D == 64 && R == 1 ? 3 : 2) void attn_qu
   // A lane holds the dims [4 kCols grp, 4 kCols (grp + 1)) of its rows.
   if constexpr (K == 1) {
     // The finished rows (keys are not cut here) go through LDS, from where the lanes write whole rows one behind
-    // the other (the epilogue of 256 rows of 128 dims: 7.9 -> 2 us).
+    // the other (the epilogue of 256 rows of 128 dims: 7.9 -> 2.5 us).
     typedef u32x4 u32x4_any __attribute__((aligned(8)));
     constexpr int kOutPitch = 2 * D + 16, kRowLanes = D / 8, kStepRows = 64 / kRowLanes;
     static_assert(kWaves * 16 * RB * kOutPitch <= kLdsBytes, "LDS of the finished rows");
@@ -853,7 +877,8 @@ __global__ __launch_bounds__(R * K * 64, D == 64 && R == 1 ? 3 : 2) void attn_qu
   }
 }
 
-// Joins the pieces of rows whose keys were cut.  D / 4 threads carry a row's dims; with many pieces `parts`
+// Joins the pieces of rows whose keys were cut (32 pieces of 32 rows of 128 dims: 4.0 us, of which the smallest launches
+// take 2.4; 18 us with one thread group per row and one piece at a time).  D / 4 threads carry a row's dims; with many pieces `parts`
 // such groups of a workgroup share a row (piece p goes to group p % parts) and are joined through LDS.  Four
 // pieces are requested at a time: the kernel is the latency of its loads.
 constexpr int kMergeThreads = 256, kMergeMaxParts = 8;
@@ -907,7 +932,8 @@ __global__ __launch_bounds__(kMergeThreads) void attn_quant_merge_kernel(QuantAr
 }
 
 // ---------------------------------------------------------------------------------------------
-// Generic kernel: one workgroup per (query, head, batch row); keys in chunks of 256.
+// Generic kernel: one workgroup per (query, head, batch row); keys in chunks of 256.  For types and head sizes that
+// no workload of this framework decodes with; each key's record is read by one lane.
 // ---------------------------------------------------------------------------------------------
 constexpr int kGenThreads = 256;
 
@@ -1003,7 +1029,8 @@ __global__ __launch_bounds__(kGenThreads) void attn_quant_generic_kernel(QuantAr
 // ---------------------------------------------------------------------------------------------
 // Within it, a run of whole units that all of them attend to in full: from the first such unit to the
 // first one behind it that is not (looked for among the first 2^15 units).  A unit's words of the queries are
-// read by as many neighbouring lanes.
+// read by as many neighbouring lanes.  Once per mask; bound by latency (two masks of 1900 x 1900: 5.1 us, one of
+// 1 x 65 537: 5.0, 1 x 33: 3.0).
 constexpr int kSpanThreads = 256, kSpanBits = 1 << 15;
 __global__ __launch_bounds__(kSpanThreads) void attn_spans_kernel(const uint64_t* __restrict__ bits, int n_q, int words,
                                                                   int kv_len, int32_t* __restrict__ spans) {
