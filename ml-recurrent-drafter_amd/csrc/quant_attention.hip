@@ -322,6 +322,7 @@ __global__ __launch_bounds__(R * K * 64, D == 64 && R == 1 ? 3 : 2) void attn_qu
   int b = blockIdx.y / a.max_pieces;
   const int piece = blockIdx.y % a.max_pieces;
   if constexpr (R > 1) {
+    static_assert(kWaves * 64 >= kMaxSorted, "a thread per pair");
     if (a.sorted) {
       __shared__ int s_pick;
       const int pair = sorted_pair(a, a.B * tiles, tiles, kRows, blockIdx.y * tiles + blockIdx.x / a.Hkv,
