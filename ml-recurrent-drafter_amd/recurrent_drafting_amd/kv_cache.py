@@ -294,6 +294,7 @@ class Cache:
             if bits not in (4, 8) or row == 0:
                 raise ValueError(f"a cache in {bits} bits with head_dim {head_dim}: bits must be 4 or 8, head_dim a "
                                  "multiple of 32 and at most 256")
+            self.bits = int(bits)
         # (the attention reads only the cache rows of keys that somebody attends to, so nothing is
         # asked of the memory around a row's live rows; zeros as upstream, kv_cache.py:49-53)
         self._storage = torch.zeros([n_layers, 2, batch_size, n_heads, max_length, row], dtype=element, device=device)
