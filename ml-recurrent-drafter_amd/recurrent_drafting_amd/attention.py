@@ -64,6 +64,7 @@ class PreparedMask:
     # which keys 16 consecutive queries attend to, as rd_attn_spans writes it: made by the first attention over
     # a cache in 4 or 8 bits that uses this mask, per stream ({stream handle, or (handle, capture): int32 tensor})
     spans: dict = field(default_factory=dict)
+    quant_workspace: dict = field(default_factory=dict)  # and its workspace bytes: {(dtype, heads, kv heads, head_dim): int}
 
 
 def prepare(mask: torch.Tensor, fix_empty_rows: bool = True, n_heads: int = 32,
@@ -211,7 +212,11 @@ def _quantized_attention(q, k, v, prepared: PreparedMask, scale, force_generic, 
     spans = _spans(prepared, stream)
     # partial results of keys cut into pieces: memory of this call alone, so that calls on several
     # streams, or captured in several graphs, may share the mask
-    ws_bytes = lib.rd_verify_attention_quant_workspace_bytes(owner.dtype_code, B, H, Hkv, n_q, kv_len, D)
+    sizes = (owner.dtype_code, H, Hkv, D)
+    ws_bytes = prepared.quant_workspace.get(sizes)
+    if ws_bytes is None:
+        ws_bytes = lib.rd_verify_attention_quant_workspace_bytes(owner.dtype_code, B, H, Hkv, n_q, kv_len, D)
+        prepared.quant_workspace[sizes] = ws_bytes
     workspace = q.new_empty(ws_bytes, dtype=torch.uint8) if ws_bytes else None
     if shape_log is not None:
         shape_log.append((B, n_q, kv_len, B * n_q if rows is None else rows.total))

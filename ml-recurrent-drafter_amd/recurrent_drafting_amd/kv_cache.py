@@ -71,21 +71,27 @@ class QuantizedRows:
     def read(self) -> torch.Tensor:
         """The values, (batch, n_heads, length - prev, head_dim) in `dtype`: exact, every value the records
         can hold is a number of that type."""
-        owner = self._owner
-        cache = owner._cache
-        batch, n_heads, n_rows, head_dim = self.shape
-        out = cache.new_empty((batch, n_heads, n_rows, head_dim), dtype=owner.dtype)
-        if n_rows == 0 or batch == 0:
-            return out
-        _hip.on_current_device(cache)
-        row = n_rows * head_dim
-        _hip.check(
-            _hip.lib().rd_kv_dequantize(
-                self.data_ptr(), owner.byte_strides, owner.bits, owner.dtype_code, batch, n_heads, 0, n_rows, head_dim,
-                n_rows, out.data_ptr(), _hip.I64x3(n_heads * row, row, head_dim), _hip.stream(),
-            )
-        )
+        return _read(self._owner, self._layer, self._kv, self._prev, self._length)
+
+
+def _read(owner: "Cache", layer: int, kv: int, prev: int, length: int) -> torch.Tensor:
+    """Rows [prev, length) of a layer's keys or values out of a cache in 4 or 8 bits (rd_kv_dequantize)."""
+    cache, head_dim, n_rows = owner._cache, owner.head_dim, length - prev
+    batch, n_heads, max_length = owner.slab_shape
+    out = cache.new_empty((batch, n_heads, n_rows, head_dim), dtype=owner.dtype)
+    if n_rows == 0 or batch == 0:
         return out
+    _hip.on_current_device(cache)
+    per_layer, per_side, _ = owner.slab_strides
+    row = n_rows * head_dim
+    _hip.check(
+        _hip.lib().rd_kv_dequantize(
+            cache.data_ptr() + layer * per_layer + kv * per_side, owner.byte_strides, owner.bits, owner.dtype_code,
+            batch, n_heads, prev, n_rows, head_dim, max_length, out.data_ptr(),
+            _hip.I64x3(n_heads * row, row, head_dim), _hip.stream(),
+        )
+    )
+    return out
 
 
 class View:
@@ -150,9 +156,12 @@ class View:
 
     def slice(self, prev: int) -> torch.Tensor:
         """Rows [prev, length) (of a cache in 4 or 8 bits: their values, read back)."""
-        if self._owner is not None:
-            self._owner.materialize()
-        return self.rows(prev) if self.bits is None else self.rows(prev).read()
+        owner = self._owner
+        if owner is not None:
+            owner.materialize()
+            if owner.bits is not None:
+                return _read(owner, self._layer, self._kv, prev, self.length)
+        return self.rows(prev)
 
 
 def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
