@@ -420,7 +420,7 @@ RD_API int rd_rope_verify_attention(const void* q, const int64_t* q_strides, con
  *
  * rd_verify_attention_quant: rd_verify_attention over such rows; mask bits, plan and row_start as
  * there.  spans: rd_attn_spans_ints(batch, n_q) int32, 16-byte aligned, written by rd_attn_spans from the
- * mask bits once per forward (for every 16 consecutive queries: the first and one past the last key that
+ * mask bits once per forward, and again whenever the bits are written (for every 16 consecutive queries: the first and one past the last key that
  * one of them attends to, and a run of keys that all of them attend to).  A row that attends to nothing
  * is written as zeros; keys nobody attends to may hold NaN blocks.  bf16 and fp16
  * with head_dim 64 or 128 (q 16-byte aligned with strides that are multiples of 8 elements, out 8-byte

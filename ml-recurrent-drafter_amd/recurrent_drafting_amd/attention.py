@@ -61,10 +61,30 @@ class PreparedMask:
     kv_len: int
     workspace: Optional[torch.Tensor] = None
     shifted: bool = False  # the plan was built with per-row cache shifts (kv_cache.Cache.shift)
-    # which keys 16 consecutive queries attend to, as rd_attn_spans writes it: made by the first attention over
-    # a cache in 4 or 8 bits that uses this mask, per stream ({stream handle, or (handle, capture): int32 tensor})
+    # which keys 16 consecutive queries attend to, as rd_attn_spans writes it, with the bits it was made from: by the
+    # attention over a cache in 4 or 8 bits, per stream ({stream handle, or (handle, capture): (int32 tensor, bits,
+    # their version)}).  See _spans.
     spans: dict = field(default_factory=dict)
     quant_workspace: dict = field(default_factory=dict)  # and its workspace bytes: {(dtype, heads, kv heads, head_dim): int}
+    # (bits, their version, the capture going on or 0) when the library wrote them; None: written by somebody else.
+    # Whoever writes them past torch (through the C ABI, or .data) sets it to None
+    written: Optional[tuple] = None
+
+
+def new_bits(words: int, device: torch.device) -> torch.Tensor:
+    """Memory for mask bits.  In inference mode too a tensor whose in-place writes torch counts."""
+    if not torch.is_inference_mode_enabled():
+        return torch.empty(words, dtype=torch.int64, device=device)
+    with torch.inference_mode(False):
+        return torch.empty(words, dtype=torch.int64, device=device)
+
+
+def prepared_mask(bits: torch.Tensor, plan: torch.Tensor, batch: int, n_q: int, kv_len: int, shifted: bool,
+                  stream: int) -> PreparedMask:
+    """The PreparedMask of bits and plan that the library has just written on `stream`, the current one."""
+    bits = bits.view(batch, n_q, -1)
+    capture = _hip.lib().rd_stream_capture_id(stream) if stream else 0
+    return PreparedMask(bits, plan, batch, n_q, kv_len, shifted=shifted, written=(bits, bits._version, capture))
 
 
 def prepare(mask: torch.Tensor, fix_empty_rows: bool = True, n_heads: int = 32,
@@ -79,16 +99,16 @@ def prepare(mask: torch.Tensor, fix_empty_rows: bool = True, n_heads: int = 32,
     assert kv_shift is None or (kv_shift.shape == (B,) and kv_shift.dtype == torch.int32 and kv_shift.is_contiguous())
     lib = _hip.lib()
     dev = mask.device
-    bits = torch.empty(lib.rd_attn_bits_words(B, n_q, kv_len), dtype=torch.int64, device=dev)
+    bits, stream = new_bits(lib.rd_attn_bits_words(B, n_q, kv_len), dev), _hip.stream()
     plan = torch.empty(lib.rd_attn_plan_ints(B, n_q, kv_len), dtype=torch.int32, device=dev)
     _hip.check(
         lib.rd_attn_prepare(
             _hip.ptr(mask), mask.stride(0), mask.stride(1), B, n_q, kv_len, int(n_heads),
             int(fix_empty_rows),
-            _hip.ptr(bits), _hip.ptr(plan), _hip.ptr(kv_shift), _hip.stream(),
+            _hip.ptr(bits), _hip.ptr(plan), _hip.ptr(kv_shift), stream,
         )
     )
-    return PreparedMask(bits.view(B, n_q, -1), plan, B, n_q, kv_len, shifted=kv_shift is not None)
+    return prepared_mask(bits, plan, B, n_q, kv_len, kv_shift is not None, stream)
 
 
 # When set to a list, every masked_attention call appends (batch, n_q, kv_len, query rows): measurement
@@ -161,21 +181,25 @@ def masked_attention(
 
 
 def _spans(prepared: PreparedMask, stream: int) -> torch.Tensor:
-    """The mask's span table, written on `stream`, the current one: kept for the later layers on that stream.
-    A table written while a graph is captured holds nothing before the replay: it is for the layers of that
-    capture."""
-    spans = prepared.spans.get(stream)
-    if spans is None:
-        lib = _hip.lib()
-        capture = lib.rd_stream_capture_id(stream)
-        key = (stream, capture) if capture else stream
-        spans = prepared.spans.get(key)
-    if spans is None:
-        spans = torch.empty(lib.rd_attn_spans_ints(prepared.batch, prepared.n_q), dtype=torch.int32,
-                            device=prepared.bits.device)
-        _hip.check(lib.rd_attn_spans(_hip.ptr(prepared.bits), prepared.batch, prepared.n_q, prepared.kv_len,
-                                     _hip.ptr(spans), stream))
-        prepared.spans[key] = spans
+    """The span table of the mask's bits as `stream`, the current one, will find them.
+
+    The layers of a forward share a table, and only they: one is read again while the bits are those that the
+    library wrote and torch has counted no write since.  Bits written inside a capture are written again by every
+    replay, and bits that somebody has written may be a static buffer, which replays write without being counted:
+    eager calls make a table of their own from these.  A capture makes its own too, so that a replay follows the
+    bits it finds."""
+    lib, bits = _hip.lib(), prepared.bits
+    capture = lib.rd_stream_capture_id(stream) if stream else 0  # (the null stream is never captured)
+    key = (stream, capture) if capture else stream
+    written = prepared.written
+    if written is not None and written[0] is bits and written[2] in (0, capture):
+        kept = prepared.spans.get(key)
+        # (in a capture the version may be a later one: the write is part of what is replayed)
+        if kept is not None and kept[1] is bits and kept[2] == bits._version and (capture or kept[2] == written[1]):
+            return kept[0]
+    spans = torch.empty(lib.rd_attn_spans_ints(prepared.batch, prepared.n_q), dtype=torch.int32, device=bits.device)
+    _hip.check(lib.rd_attn_spans(_hip.ptr(bits), prepared.batch, prepared.n_q, prepared.kv_len, _hip.ptr(spans), stream))
+    prepared.spans[key] = (spans, bits, None if bits.is_inference() else bits._version)
     return spans
 
 

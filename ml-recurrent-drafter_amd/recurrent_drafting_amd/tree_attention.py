@@ -163,7 +163,7 @@ def prepare_attention(tree: PackedTree, padding_mask: torch.Tensor, pad_value: i
     n, kv_len = tree.n, prev + tree.n
     lib = _hip.lib()
     dev = tree.unpacker.device
-    bits = torch.empty(lib.rd_attn_bits_words(B, n, kv_len), dtype=torch.int64, device=dev)
+    bits, stream = attention.new_bits(lib.rd_attn_bits_words(B, n, kv_len), dev), _hip.stream()
     plan = torch.empty(lib.rd_attn_plan_ints(B, n, kv_len), dtype=torch.int32, device=dev)
     position_ids = torch.empty((B, n), dtype=torch.long, device=dev)
     left_pads = torch.empty(B, dtype=torch.int32, device=dev)
@@ -173,10 +173,10 @@ def prepare_attention(tree: PackedTree, padding_mask: torch.Tensor, pad_value: i
             _hip.ptr(padding_mask) if prev > 0 else None, padding_mask.element_size(),
             padding_mask.stride(0) if prev > 0 else 0, int(pad_value), prev, B, W, L, n, int(n_heads),
             _hip.ptr(bits), _hip.ptr(plan), _hip.ptr(position_ids), _hip.ptr(left_pads), _hip.ptr(kv_shift),
-            _hip.stream(),
+            stream,
         )
     )
-    return attention.PreparedMask(bits.view(B, n, -1), plan, B, n, kv_len, shifted=kv_shift is not None), position_ids, left_pads
+    return attention.prepared_mask(bits, plan, B, n, kv_len, kv_shift is not None, stream), position_ids, left_pads
 
 
 def pack(
