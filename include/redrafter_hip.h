@@ -429,7 +429,7 @@ RD_API int rd_rope_verify_attention(const void* q, const int64_t* q_strides, con
  * none is needed, NULL will do), 256-byte aligned; each call needs one of its own while it runs.  Nothing
  * in the library is shared between calls.  scale must be positive.  Rows of one slab must follow each
  * other without gaps (cache_strides[2] = the record).  Limits: kv_len <= 2^23,
- * n_q * n_heads / n_kv_heads <= 2^30. */
+ * n_q * n_heads / n_kv_heads <= 2^30; 2^8 |v| summed over the keys of a row stays below fp32's largest number. */
 RD_API size_t rd_kv_quant_row_bytes(int bits, int head_dim);
 RD_API int rd_rope_append_quant(const void* q, const int64_t* q_strides, const void* k,
                                 const int64_t* k_strides, const void* v, const int64_t* v_strides,

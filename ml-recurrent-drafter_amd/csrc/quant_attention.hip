@@ -19,13 +19,14 @@
 //                accumulators of the first product into the B operand of the second as it is.
 //                Codes of two keys become two dims times two keys: two conversions (code pair x scale
 //                to a 16-bit pair, one instruction, exact) and two byte permutes.
-// P is rounded to the 16-bit type there (half a step of it, 2^-9 or 2^-12 of a weight, as every 16-bit product
-// of the model rounds); scores, maximum, sums and accumulators are fp32.  The row sums come out of the
+// P is rounded to the 16-bit type there (half a step of it, as every 16-bit product of the model rounds: 2^-9 of a
+// weight in bf16; in fp16 2^-12, and for weights below 2^-21 of the running maximum's 2^-32 of that one); scores, maximum, sums and accumulators are fp32.  The row sums come out of the
 // matrix pipeline too, as the product of P with ones: the sum of the rounded weights, the ones that V is
 // multiplied with.
 // A query row lives in one column of the accumulators (l % 16), so rescaling is a lane scalar; the running
 // maximum is lazy: raised only when some score exceeds it by 2^8 in the exponential, where fp32 has room
-// for 2^120 such weights.
+// for 2^120 such weights (values times weights are summed before they are divided: 2^8 |v| summed over a row's
+// keys has to be a finite number of fp32, which only values beyond 2^97 or so can miss).
 //
 // Records travel memory -> registers (whole contiguous units, 16 bytes per lane) -> LDS as they lie in
 // memory, and are picked apart from there without a bank conflict (rows of 48, 80 and 144 bytes spread 16
@@ -102,6 +103,7 @@ template <> struct Ops<__hip_bfloat16> {
   using V8 = bf16x8;
   static constexpr bool kF16 = false;
   static constexpr uint32_t kOne = 0x3f80u;
+  static constexpr float kLift = 0.f;              // (see weights)
   static __device__ uint32_t fp4(uint32_t w, float s, std::integral_constant<int, 0>) { return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 0)); }
   static __device__ uint32_t fp4(uint32_t w, float s, std::integral_constant<int, 1>) { return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 1)); }
   static __device__ uint32_t fp4(uint32_t w, float s, std::integral_constant<int, 2>) { return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 2)); }
@@ -120,6 +122,7 @@ template <> struct Ops<__half> {
   using V8 = f16x8;
   static constexpr bool kF16 = true;
   static constexpr uint32_t kOne = 0x3c00u;
+  static constexpr float kLift = 7.f;
   static __device__ uint32_t fp4(uint32_t w, float s, std::integral_constant<int, 0>) { return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 0)); }
   static __device__ uint32_t fp4(uint32_t w, float s, std::integral_constant<int, 1>) { return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 1)); }
   static __device__ uint32_t fp4(uint32_t w, float s, std::integral_constant<int, 2>) { return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 2)); }
@@ -614,7 +617,10 @@ __global__ __launch_bounds__(R * K * 64, D == 64 && R == 1 ? 3 : 2) void attn_qu
 #pragma unroll
         for (int j = 0; j < kCols; ++j) o[rb][j] *= keep;
       }
-      const float m_use = fmaxf(m[rb], -3.4e38f);   // nothing attended yet: every p below is exp2(-inf)
+      // nothing attended yet: every p below is exp2(-inf).  fp16 weights are held 2^7 times as large, 2^15 at most: its
+      // smallest number is 2^-24, and 2^23 keys of 2^-26 of the largest weight are an eighth of the sum.  The sum has
+      // the factor too, and so the quotient has not.
+      const float m_use = fmaxf(m[rb], -3.4e38f) - O::kLift;
       float p[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) p[j] = fast_exp2(__builtin_fmaf(x[j], a.scale, -m_use));
