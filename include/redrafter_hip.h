@@ -410,8 +410,8 @@ RD_API int rd_rope_verify_attention(const void* q, const int64_t* q_strides, con
  * other by rd_kv_unpack, rd_kv_compact, rd_kv_append and rd_kv_materialize with row_bytes = the record;
  * below, cache_strides are HOST arrays of BYTE strides {batch, head, row}.
  *
- * rd_rope_append_quant: rd_rope_append into such rows.  k is rotated without intermediate rounding and
- * the record is that of the exact rotated key; q_out is the rotated q rounded once (rd_rope_append
+ * rd_rope_append_quant: rd_rope_append into such rows.  k is rotated in fp64 (exact products, one
+ * rounded sum) and the record is that of the sum; q_out is the rotated q rounded once (rd_rope_append
  * rounds every product).  All other arguments as for rd_rope_append.
  * rd_kv_quantize: rows x (batch, n_kv_heads, n_rows, head_dim), HOST element strides {batch, head, row},
  * last dimension contiguous, into the cache rows [row0, row0 + n_rows) of one layer's keys or values.

@@ -179,7 +179,7 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Te
     The cache still grows by n rows per batch row (the slots that do not exist keep what the
     cache held), and q comes back as a (total, heads, D) view.
 
-    A cache in 4 or 8 bits takes the records of the exact rotated keys and of the values, and keys and
+    A cache in 4 or 8 bits takes the records of the keys as fp64 rotates them and of the values, and keys and
     values come back as its `QuantizedRows`.  q is then rotated into a tensor of its own (rounded once; the
     projection's output is left as it was), of which the result is a view; rows behind the last token of
     a packed batch are not written."""
