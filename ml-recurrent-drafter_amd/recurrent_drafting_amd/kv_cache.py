@@ -36,7 +36,8 @@ class QuantizedRows:
     __slots__ = ("_owner", "_layer", "_kv", "_prev", "_length")
 
     def __init__(self, owner: "Cache", layer: int, kv: int, prev: int, length: int):
-        self._owner, self._layer, self._kv, self._prev, self._length = owner, layer, kv, prev, length
+        # (prev behind the last row: no rows, as of a tensor's slice)
+        self._owner, self._layer, self._kv, self._prev, self._length = owner, layer, kv, min(prev, length), length
 
     @property
     def bits(self) -> int:
@@ -76,7 +77,7 @@ class QuantizedRows:
 
 def _read(owner: "Cache", layer: int, kv: int, prev: int, length: int) -> torch.Tensor:
     """Rows [prev, length) of a layer's keys or values out of a cache in 4 or 8 bits (rd_kv_dequantize)."""
-    cache, head_dim, n_rows = owner._cache, owner.head_dim, length - prev
+    cache, head_dim, n_rows = owner._cache, owner.head_dim, max(length - prev, 0)
     batch, n_heads, max_length = owner.slab_shape
     out = cache.new_empty((batch, n_heads, n_rows, head_dim), dtype=owner.dtype)
     if n_rows == 0 or batch == 0:

@@ -1,0 +1,19 @@
+"""Edges of the 4- and 8-bit cache's calls that the host answers."""
+import pytest
+import torch
+
+
+@pytest.mark.parametrize("bits", [None, 4, 8])
+def test_a_slice_behind_the_last_row_is_empty(bits):
+    """As of a cache in the model's type."""
+    from recurrent_drafting_amd import kv_cache
+
+    cache = kv_cache.Cache(2, 6, 1, 3, 64, torch.bfloat16, torch.device("cpu"), bits=bits)
+    key, _ = cache.sliced[0]
+    key.length = 2
+    for prev in (2, 3, 6, 9):
+        got = key.slice(prev)
+        assert got.shape == (2, 3, 0, 64) and got.dtype == torch.bfloat16
+        assert key.rows(prev).shape == (2, 3, 0, 64)
+    if bits is not None:
+        assert key.rows(9).read().shape == (2, 3, 0, 64) and key.rows(9).records.shape[2] == 0
