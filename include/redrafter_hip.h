@@ -427,7 +427,7 @@ RD_API int rd_rope_verify_attention(const void* q, const int64_t* q_strides, con
  * aligned with strides that are multiples of 4) run on the MFMA kernel, everything else, or
  * force_generic != 0, on the generic kernel.  workspace: rd_verify_attention_quant_workspace_bytes (0:
  * none is needed, NULL will do), 256-byte aligned; each call needs one of its own while it runs.  Nothing
- * in the library is shared between calls.  scale must be positive.  Rows of one slab must follow each
+ * in the library is shared between calls.  scale must be positive, and finite times log2(e).  Rows of one slab must follow each
  * other without gaps (cache_strides[2] = the record).  Limits: kv_len <= 2^23,
  * n_q * n_heads / n_kv_heads <= 2^30; 2^8 |v| summed over the keys of a row stays below fp32's largest number. */
 RD_API size_t rd_kv_quant_row_bytes(int bits, int head_dim);

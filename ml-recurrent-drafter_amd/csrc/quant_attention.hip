@@ -1248,7 +1248,9 @@ extern "C" int rd_verify_attention_quant(const void* q, const int64_t* q_strides
   RD_REQUIRE(q && k_cache && v_cache && out && mask_bits && plan && spans && q_strides && cache_strides && o_strides,
              RD_EINVAL, "%s: null pointer", who);
   RD_REQUIRE(max_len > 0, RD_EINVAL, "%s: empty cache", who);
-  RD_REQUIRE(scale > 0.f && scale <= 3.402823466e38f, RD_EINVAL, "%s: scale %g is not a positive finite number", who, (double)scale);
+  // (scores are held in log2 units)
+  RD_REQUIRE(scale > 0.f && scale * 1.4426950408889634f <= 3.402823466e38f, RD_EINVAL,
+             "%s: scale %g is not positive, or times log2(e) not finite", who, (double)scale);
   auto al = [](const void* p, int n) { return ((uintptr_t)p & (n - 1)) == 0; };
   RD_REQUIRE(al(k_cache, 16) && al(v_cache, 16) && al(spans, 16), RD_EINVAL, "%s: the cache and the spans must be 16-byte aligned", who);
   RD_REQUIRE(cache_strides[0] % 16 == 0 && cache_strides[1] % 16 == 0 && cache_strides[0] >= 0 && cache_strides[1] >= 0 &&
