@@ -61,9 +61,9 @@ class PreparedMask:
     kv_len: int
     workspace: Optional[torch.Tensor] = None
     shifted: bool = False  # the plan was built with per-row cache shifts (kv_cache.Cache.shift)
-    # which keys 16 consecutive queries attend to, as rd_attn_spans writes it, with the bits it was made from: by the
-    # attention over a cache in 4 or 8 bits, per stream ({stream handle, or (handle, capture): (int32 tensor, bits,
-    # their version)}).  See _spans.
+    # which keys 16 consecutive queries attend to, as rd_attn_spans writes it, with what it was made from: by the
+    # attention over a cache in 4 or 8 bits, per stream ({stream handle, or (handle, capture): (int32 tensor, `written`,
+    # bits, their version)}).  See _spans.
     spans: dict = field(default_factory=dict)
     quant_workspace: dict = field(default_factory=dict)  # and its workspace bytes: {(dtype, heads, kv heads, head_dim): int}
     # (bits, their version, the capture going on or 0) when the library wrote them; None: written by somebody else.
@@ -180,6 +180,9 @@ def masked_attention(
     return out.view(B, n_q, H * D) if rows is None else out.view(rows.rows, H * D)
 
 
+_never = object()  # in the place of `written`: a table that is not read again
+
+
 def _spans(prepared: PreparedMask, stream: int) -> torch.Tensor:
     """The span table of the mask's bits as `stream`, the current one, will find them.
 
@@ -188,18 +191,19 @@ def _spans(prepared: PreparedMask, stream: int) -> torch.Tensor:
     replay, and bits that somebody has written may be a static buffer, which replays write without being counted:
     eager calls make a table of their own from these.  A capture makes its own too, so that a replay follows the
     bits it finds."""
-    lib, bits = _hip.lib(), prepared.bits
-    capture = lib.rd_stream_capture_id(stream) if stream else 0  # (the null stream is never captured)
+    bits, written = prepared.bits, prepared.written
+    capture = _hip.lib().rd_stream_capture_id(stream) if stream else 0  # (the null stream is never captured)
     key = (stream, capture) if capture else stream
-    written = prepared.written
-    if written is not None and written[0] is bits and written[2] in (0, capture):
-        kept = prepared.spans.get(key)
-        # (in a capture the version may be a later one: the write is part of what is replayed)
-        if kept is not None and kept[1] is bits and kept[2] == bits._version and (capture or kept[2] == written[1]):
-            return kept[0]
+    kept = prepared.spans.get(key)
+    if kept is not None and kept[1] is written and kept[2] is bits and kept[3] == bits._version:
+        return kept[0]
+    lib = _hip.lib()
     spans = torch.empty(lib.rd_attn_spans_ints(prepared.batch, prepared.n_q), dtype=torch.int32, device=bits.device)
     _hip.check(lib.rd_attn_spans(_hip.ptr(bits), prepared.batch, prepared.n_q, prepared.kv_len, _hip.ptr(spans), stream))
-    prepared.spans[key] = (spans, bits, None if bits.is_inference() else bits._version)
+    # (in a capture the version may be a later one: the write is part of what is replayed)
+    again = written is not None and written[0] is bits and written[2] in (0, capture) and \
+        (capture != 0 or written[1] == bits._version)
+    prepared.spans[key] = (spans, written, bits, bits._version) if again else (spans, _never, bits, None)
     return spans
 
 
@@ -224,8 +228,8 @@ def _quantized_attention(q, k, v, prepared: PreparedMask, scale, force_generic, 
     strides, address = q.stride(), q.data_ptr()
     # Rows off the 16-byte grid are copied onto it for the MFMA kernel, which reads nothing else (8 x 32 heads, 115
     # queries, 735 keys: 36 us aligned, 39 with the copy, 6.5 ms on the generic kernel).
-    off_grid = not force_generic and D in (64, 128) and owner.dtype != torch.float32 and \
-        (address | 2 * strides[0] | 2 * strides[1] | 2 * strides[-2]) & 15
+    off_grid = (address | (strides[0] | strides[1] | strides[-2]) << 1) & 15 and D in (64, 128) and \
+        owner.dtype != torch.float32 and not force_generic
     if strides[-1] != 1 or off_grid:
         q = q.clone(memory_format=torch.contiguous_format)
         strides, address = q.stride(), q.data_ptr()

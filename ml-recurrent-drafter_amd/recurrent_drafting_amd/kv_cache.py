@@ -37,7 +37,8 @@ class QuantizedRows:
 
     def __init__(self, owner: "Cache", layer: int, kv: int, prev: int, length: int):
         # (prev behind the last row: no rows, as of a tensor's slice)
-        self._owner, self._layer, self._kv, self._prev, self._length = owner, layer, kv, min(prev, length), length
+        self._owner, self._layer, self._kv, self._length = owner, layer, kv, length
+        self._prev = prev if prev < length else length
 
     @property
     def bits(self) -> int:
