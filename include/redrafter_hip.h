@@ -420,16 +420,17 @@ RD_API int rd_rope_verify_attention(const void* q, const int64_t* q_strides, con
  *
  * rd_verify_attention_quant: rd_verify_attention over such rows; mask bits, plan and row_start as
  * there.  spans: rd_attn_spans_ints(batch, n_q) int32, 16-byte aligned, written by rd_attn_spans from the
- * mask bits once per forward, and again whenever the bits are written (for every 16 consecutive queries: the first and one past the last key that
- * one of them attends to, and a run of keys that all of them attend to).  A row that attends to nothing
- * is written as zeros; keys nobody attends to may hold NaN blocks.  bf16 and fp16
+ * mask bits, once per forward and again whenever the bits are written (for every 16 consecutive queries:
+ * the first and one past the last key that one of them attends to, and a run of keys that all of them
+ * attend to; with the spans of other bits keys are dropped and masked ones attended to).  A row that
+ * attends to nothing is written as zeros; keys nobody attends to may hold NaN blocks.  bf16 and fp16
  * with head_dim 64 or 128 (q 16-byte aligned with strides that are multiples of 8 elements, out 8-byte
  * aligned with strides that are multiples of 4) run on the MFMA kernel, everything else, or
  * force_generic != 0, on the generic kernel.  workspace: rd_verify_attention_quant_workspace_bytes (0:
  * none is needed, NULL will do), 256-byte aligned; each call needs one of its own while it runs.  Nothing
- * in the library is shared between calls.  scale must be positive, and finite times log2(e).  Rows of one slab must follow each
- * other without gaps (cache_strides[2] = the record).  Limits: kv_len <= 2^23,
- * n_q * n_heads / n_kv_heads <= 2^30; 2^8 |v| summed over the keys of a row stays below fp32's largest number. */
+ * in the library is shared between calls.  scale must be positive, and finite times log2(e).  Rows of
+ * one slab must follow each other without gaps (cache_strides[2] = the record).  Limits: kv_len <= 2^23,
+ * n_q * n_heads / n_kv_heads <= 2^30; 2^8 |v| summed over the keys of a row stays below fp32's largest. */
 RD_API size_t rd_kv_quant_row_bytes(int bits, int head_dim);
 RD_API int rd_rope_append_quant(const void* q, const int64_t* q_strides, const void* k,
                                 const int64_t* k_strides, const void* v, const int64_t* v_strides,

@@ -15,8 +15,9 @@
 //
 // Record of a row: D * bits / 8 code bytes, then D / 8 scale bytes, padded to a multiple of 16 bytes
 // (rows stay whole 16-byte units for the row movement kernels).  D = 128: 80 and 144 bytes, where
-// bf16 takes 256.  Blocks of 8 instead of 32 cost nothing there (the scale bytes fill what would be
-// padding) and gain 0.5 to 1.7 dB of signal to rounding noise at 4 bits.
+// bf16 takes 256.  Blocks of 8 instead of 32 cost no bytes there (the scale bytes fill what would be
+// padding) and gain 0.5 to 1.7 dB of signal to rounding noise at 4 bits; what they cost is the matrix instructions that
+// apply one scale to 32 values, for which queries and weights would have to be rounded to 8 bits or fewer as well.
 #pragma once
 
 #include <stddef.h>
