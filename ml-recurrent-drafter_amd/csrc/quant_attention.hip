@@ -27,6 +27,8 @@
 // maximum is lazy: raised only when some score exceeds it by 2^8 in the exponential, where fp32 has room
 // for 2^120 such weights (values times weights are summed before they are divided: 2^8 |v| summed over a row's
 // keys has to be a finite number of fp32, which only values beyond 2^97 or so can miss).
+// Weights depend on differences of scores alone: where a row's maximum is so large that its rounding in log2 units
+// matters (2^22), the keys are gone over once more with the scores subtracted before they are scaled.
 //
 // Records travel memory -> registers (whole contiguous units, 16 bytes per lane) -> LDS as they lie in
 // memory, and are picked apart from there without a bank conflict (rows of 48, 80 and 144 bytes spread 16
@@ -79,6 +81,7 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kUnit = 32;        // keys a wave takes at a time
 constexpr int kSpanQueries = 16; // queries that share an entry of the span table
+constexpr float kFar = 4194304.f;  // 2^22: fp32 has a quarter of a unit there
 constexpr int kSpanInts = 4;     // {first key, one past the last, full_lo, full_hi} of those queries
 
 struct QuantArgs {
@@ -94,6 +97,7 @@ struct QuantArgs {
   int sorted;      // workgroups take their tiles by rank (sorted_pair)
   float scale;     // softmax scale; times log2 e for the MFMA kernel
   float inv_scale; // its reciprocal
+  float rise;      // how far a score may lie above the running maximum: 8 in log2 units
 };
 
 __device__ inline float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -538,7 +542,7 @@ __global__ __launch_bounds__(R * K * 64, D == 64 && R == 1 ? 3 : 2) void attn_qu
   const bool active = row0 + 16 * RB * row_wave < t.rows;  // (a wave without rows only brings and converts units)
 
   // o: output tiles, l: row sums (the product of P with ones: every element of a lane's l is its row's sum),
-  // m: running maximum in log2 units, over: the score above which it is raised
+  // m: running maximum in log2 units, over: the score above which it is raised (second sweep: the score of m)
   f32x4 o[RB][kCols], l[RB];
   float m[RB], over[RB];
   float inf = INFINITY;
@@ -591,8 +595,10 @@ __global__ __launch_bounds__(R * K * 64, D == 64 && R == 1 ? 3 : 2) void attn_qu
     }
   };
   // Scores to weights.  sc[rb][h] holds keys 16 h + 4 grp + e of row `col`; the weights come out in the order
-  // of the second product's B operand.
-  auto weights = [&](f32x4 (&sc)[RB][2], bool full, const uint32_t (&on)[RB], u32x4 (&pf)[RB]) __attribute__((always_inline)) {
+  // of the second product's B operand.  kCheck: scores are subtracted before they are scaled (one instruction more per
+  // weight), so that the rounding of a large m in log2 units is no factor of the row's weights.
+  auto weights = [&](auto check_c, f32x4 (&sc)[RB][2], bool full, const uint32_t (&on)[RB], u32x4 (&pf)[RB]) __attribute__((always_inline)) {
+    constexpr bool kCheck = decltype(check_c)::value;
     if (!full) {
 #pragma unroll
       for (int rb = 0; rb < RB; ++rb) {
@@ -608,11 +614,12 @@ __global__ __launch_bounds__(R * K * 64, D == 64 && R == 1 ? 3 : 2) void attn_qu
 #pragma unroll
       for (int j = 0; j < 8; ++j) x[j] = sc[rb][j / 4][j % 4];
       const float top = fmaxf(fmaxf(larger(x[0], x[1], inf), larger(x[2], x[3], inf)), fmaxf(larger(x[4], x[5], inf), larger(x[6], x[7], inf)));
-      if (__ballot(top > over[rb]) != 0) {
-        const float up = fmaxf(m[rb], row_max(top) * a.scale);
+      if (__ballot(kCheck ? top - over[rb] > a.rise : top > over[rb]) != 0) {
+        const float raw = kCheck ? fmaxf(over[rb], row_max(top)) : 0.f;
+        const float up = kCheck ? raw * a.scale : fmaxf(m[rb], row_max(top) * a.scale);
         const float keep = up == -INFINITY ? 1.f : fast_exp2(m[rb] - up);
         m[rb] = up;
-        over[rb] = (up + 8.f) * a.inv_scale;
+        over[rb] = kCheck ? raw : (up + 8.f) * a.inv_scale;
         l[rb] *= keep;
 #pragma unroll
         for (int j = 0; j < kCols; ++j) o[rb][j] *= keep;
@@ -620,10 +627,10 @@ __global__ __launch_bounds__(R * K * 64, D == 64 && R == 1 ? 3 : 2) void attn_qu
       // nothing attended yet: every p below is exp2(-inf).  fp16 weights are held 2^7 times as large, 2^15 at most: its
       // smallest number is 2^-24, and 2^23 keys of 2^-26 of the largest weight are an eighth of the sum.  The sum has
       // the factor too, and so the quotient has not.
-      const float m_use = fmaxf(m[rb], -3.4e38f) - O::kLift;
+      const float m_use = fmaxf(kCheck ? over[rb] : m[rb], -3.4e38f) - (kCheck ? 0.f : O::kLift);
       float p[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) p[j] = fast_exp2(__builtin_fmaf(x[j], a.scale, -m_use));
+      for (int j = 0; j < 8; ++j) p[j] = fast_exp2(kCheck ? __builtin_fmaf(x[j] - m_use, a.scale, O::kLift) : __builtin_fmaf(x[j], a.scale, -m_use));
       pf[rb] = u32x4{O::pack(p[0], p[1]), O::pack(p[2], p[3]), O::pack(p[4], p[5]), O::pack(p[6], p[7])};
     }
   };
@@ -677,7 +684,7 @@ __global__ __launch_bounds__(R * K * 64, D == 64 && R == 1 ? 3 : 2) void attn_qu
         __builtin_amdgcn_s_setprio(0);
         if constexpr (kCheck) part_nan(c, on);
         u32x4 pf[RB];
-        weights(sc, full, on, pf);
+        weights(check_c, sc, full, on, pf);
         const VPairs pairs = v_pairs(c);
         if (i + kWaves < n_units) next(i + kWaves);
         __builtin_amdgcn_sched_barrier(0);
@@ -761,7 +768,7 @@ __global__ __launch_bounds__(R * K * 64, D == 64 && R == 1 ? 3 : 2) void attn_qu
           }
           u32x4 pf[RB];
           __builtin_amdgcn_s_setprio(0);
-          weights(sc, full, on, pf);
+          weights(check_c, sc, full, on, pf);
           __builtin_amdgcn_s_setprio(1);
           if constexpr (!kCheck) {
             const u32x4* const ready = reinterpret_cast<const u32x4*>(here) + lane;
@@ -784,8 +791,12 @@ __global__ __launch_bounds__(R * K * 64, D == 64 && R == 1 ? 3 : 2) void attn_qu
   };
   sweep(std::false_type{});
   // A NaN in the output comes from one that somebody attends to, or from a NaN block of V under a masked
-  // key (0 * NaN): the wave goes over its keys once more and keeps the two apart.
+  // key (0 * NaN): the wave goes over its keys once more and keeps the two apart.  So it does where a row's
+  // maximum is so large that its rounding, a factor of all the row's weights, can leave the type's range (finite scores of
+  // 2^28 in log2 units gave NaN or zeros); in the loop of the first sweep that would cost 2 to 10 % of every launch.
   bool odd_row = false;
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) odd_row = odd_row || (fabsf(m[rb]) > kFar && m[rb] != -INFINITY);
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
@@ -1269,7 +1280,7 @@ extern "C" int rd_verify_attention_quant(const void* q, const int64_t* q_strides
   a.span_blocks = (int)rd::ceil_div(n_q, kSpanQueries);
   a.sorted = 0;
   a.max_pieces = 1; a.piece = (int)(rd::ceil_div((int64_t)kv_len + kUnit - 1, kUnit) * kUnit);
-  a.scale = scale; a.inv_scale = 1.f;
+  a.scale = scale; a.inv_scale = 1.f; a.rise = 0.f;
   hipStream_t s = rd::as_stream(stream);
   auto whole = [](const int64_t* st, int m) { return st[0] % m == 0 && st[1] % m == 0 && st[2] % m == 0; };
   const bool mfma = !force_generic && mfma_shape(dtype, head_dim) && al(q, 16) && al(out, 8) && whole(q_strides, 8) && whole(o_strides, 4);
@@ -1281,6 +1292,8 @@ extern "C" int rd_verify_attention_quant(const void* q, const int64_t* q_strides
     a.sorted = sh.sorted;
     a.scale = scale * 1.4426950408889634f;
     a.inv_scale = 1.f / a.scale;
+    a.rise = 8.f / a.scale;
+    if (!(a.rise <= 3.402823466e38f)) a.rise = 3.402823466e38f;  // (less than from no score at all, -infinity, to one)
     if (sh.max_pieces > 1) {
       const size_t need = rd_verify_attention_quant_workspace_bytes(dtype, batch, n_heads, n_kv_heads, n_q, kv_len, head_dim);
       RD_REQUIRE(workspace && workspace_bytes >= need, RD_EWORKSPACE, "%s: workspace %zu < %zu bytes", who, workspace_bytes, need);
